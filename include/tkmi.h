@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define TKMI_ABI_VERSION 5
+#define TKMI_ABI_VERSION 6
 
 typedef uint16_t tk_half;
 
@@ -38,7 +38,7 @@ enum tk_status {
   TK_ERR_HIP = -3          /* the HIP runtime rejected the launch          */
 };
 
-enum tk_dtype { TK_F32 = 0, TK_F16 = 1 };
+enum tk_dtype { TK_F32 = 0, TK_F16 = 1, TK_BF16 = 2 /* the serving calls at the end only */ };
 
 /*
  * Padding masks.  `row_valid` arguments are nullable [rows] byte arrays
@@ -436,6 +436,127 @@ const char *tk_forward_step_name(const tk_model *model, int64_t batch, int64_t s
 int tk_forward(const tk_model *model, const void *x, void *out, int64_t batch, int64_t seq,
                const uint8_t *valid, void *workspace, int64_t workspace_bytes, int flags,
                int64_t first_step, int64_t num_steps, void *stream);
+
+/*
+ * Serving: attention over a window of keys, a paged key/value cache, and attention of one
+ * new token over it.  All of them take 16-bit tensors of one dtype (TK_F16 or TK_BF16),
+ * head_dim a multiple of 8 up to 256, and rows of 16-byte vectors (base 16-byte aligned,
+ * strides multiples of 8 elements; out: 8-byte in tk_window_attn, any in tk_paged_attn).
+ * heads is a multiple of kv_heads; head h reads key head h / (heads / kv_heads).
+ * No counterpart in the reference, which recomputes whole sequences with full causal
+ * attention (src/kernels.py:250-294).
+ */
+
+/*
+ * Causal attention of the last q_len of k_len positions (q_len <= k_len): query i sits at
+ * position p = k_len - q_len + i and sees key j when j <= p, and j > p - window or
+ * j < sinks, and key_valid[b * key_valid_stride + j] (nullable) is set.  window >= 1; one of
+ * k_len or more is plain causal attention.  A query that sees nothing gets 0.
+ * q [batch, heads, q_len, head_dim], k and v [batch, kv_heads, k_len, head_dim], out as q:
+ * element strides {b, h, s} in *_strides[3].  scale > 0.  What K and V hold at keys that
+ * are not valid has no effect; at valid ones it must be finite.
+ */
+int tk_window_attn(const void *q, const int64_t *q_strides, const void *k,
+                   const int64_t *k_strides, const void *v,
+                   const int64_t *v_strides, void *out,
+                   const int64_t *o_strides, int dtype, int64_t batch,
+                   int64_t heads, int64_t kv_heads, int64_t q_len,
+                   int64_t k_len, int64_t head_dim, float scale,
+                   int64_t window, int64_t sinks, const uint8_t *key_valid,
+                   int64_t key_valid_stride, void *stream);
+
+/*
+ * The cache: k and v pages [layers][pages][kv_heads][page_size][head_dim] (any strides with
+ * 16-byte rows; page_size a power of two from 16 to 1024) and three int32 arrays on the
+ * device: table [rows][table_width], row stride table_stride; lengths [rows]; refs [pages].
+ * A sequence of n tokens holds the first ceil(n / page_size) entries of its row, token j in
+ * row j % page_size of page table[j / page_size].  refs counts the sequences that hold a
+ * page; it is free at refs <= 0.  Entries that are no page of the cache are never followed.
+ */
+
+/*
+ * out[b, h] = attention of the token at position lengths[b] - 1 over sequence b: q
+ * [batch, heads, head_dim], strides {b, h}; pages of one layer, strides {page, head, row}.
+ * It sees key j when j >= lengths[b] - window or j < sinks; window 0: every key.  Keys whose
+ * table entry is no page of the cache are not seen; a sequence that sees nothing gets 0.
+ * max_length: the longest length to be expected; it only sizes the split of the keys over
+ * workgroups, longer sequences are attended whole.  batch_invariant: a sequence's bits do
+ * not depend on the rest of the batch or on max_length, which then counts (in the workspace's
+ * size too) as at least table_width * page_size.  workspace: tk_paged_attn_workspace bytes, 16-byte
+ * aligned, this call's own until its launches have run (0 bytes: may be NULL).
+ */
+int64_t tk_paged_attn_workspace(int64_t batch, int64_t heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t max_length,
+                                int64_t window, int64_t sinks,
+                                int batch_invariant);
+int tk_paged_attn(const void *q, const int64_t *q_strides, const void *k_pages,
+                  const int64_t *k_strides, const void *v_pages,
+                  const int64_t *v_strides, void *out,
+                  const int64_t *o_strides, int dtype, int64_t batch,
+                  int64_t heads, int64_t kv_heads, int64_t head_dim,
+                  int64_t pages, int64_t page_size, const int32_t *table,
+                  int64_t table_stride, int64_t table_width,
+                  const int32_t *lengths, int64_t max_length, float scale,
+                  int64_t window, int64_t sinks, int batch_invariant,
+                  void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Writes the last added[b] tokens (nullable: n; at most n) of every sequence into its pages:
+ * row i < added[b] of k and v [batch, n, kv_heads, head_dim], strides {b, token, head}, goes
+ * to position lengths[b] - added[b] + i.  Positions before 0, past the table, or on an entry
+ * that is no page of the cache are left out.  Pages of one layer, strides {page, head, row}.
+ */
+int tk_cache_append(const void *k, const int64_t *k_strides, const void *v,
+                    const int64_t *v_strides, void *k_pages,
+                    const int64_t *k_page_strides, void *v_pages,
+                    const int64_t *v_page_strides, int64_t batch, int64_t n,
+                    int64_t kv_heads, int64_t head_dim, int64_t pages,
+                    int64_t page_size, const int32_t *table,
+                    int64_t table_stride, int64_t table_width,
+                    const int32_t *lengths, const int32_t *added, void *stream);
+
+/*
+ * Page bookkeeping, decided on the device.  An operation that cannot be done whole changes
+ * nothing and leaves the reason in *status (device): the number of pages that were missing,
+ * or -1 for a row, length or count that cannot be taken; 0 when done.  Free pages are taken
+ * from the lowest id on.  workspace: tk_cache_workspace bytes (rows, pages, and n children;
+ * n = 0 but for a fork), 4-byte aligned, this call's own until its launches have run.
+ *
+ * reserve: lengths[b] += added[b] >= 0 for every row, with the pages that this needs.
+ * fork:    child i (an empty row, named once) becomes a copy of parent i as it was before the
+ *          call: it shares the parent's whole pages and gets a page of its own with the rows
+ *          of the one that is begun, in every layer (strides {layer, page, head, row}).
+ * free:    every listed row gives up its pages (-1 in the table) and has length 0; rows that
+ *          are not in the table are passed over, a row listed twice is freed once.
+ * compact: with `used` live pages in all, the i-th live page of those with id >= used moves
+ *          into the i-th free one below, ascending, in every layer; table and refs follow.
+ *          *used (device): their number, so that pages [used, pages) are free afterwards.
+ */
+int64_t tk_cache_workspace(int64_t rows, int64_t pages, int64_t n);
+int tk_cache_reserve(int32_t *table, int64_t table_stride, int64_t table_width,
+                     int64_t rows, int32_t *lengths, int32_t *refs,
+                     int64_t pages, int64_t page_size, const int32_t *added,
+                     int32_t *status, void *workspace, int64_t workspace_bytes,
+                     void *stream);
+int tk_cache_fork(void *k_pages, const int64_t *k_strides, void *v_pages,
+                  const int64_t *v_strides, int64_t layers, int64_t kv_heads,
+                  int64_t head_dim, int32_t *table, int64_t table_stride,
+                  int64_t table_width, int64_t rows, int32_t *lengths,
+                  int32_t *refs, int64_t pages, int64_t page_size,
+                  const int32_t *parents, const int32_t *children, int64_t n,
+                  int32_t *status, void *workspace, int64_t workspace_bytes,
+                  void *stream);
+int tk_cache_free(int32_t *table, int64_t table_stride, int64_t table_width,
+                  int64_t rows, int32_t *lengths, int32_t *refs, int64_t pages,
+                  int64_t page_size, const int32_t *list, int64_t n,
+                  void *stream);
+int tk_cache_compact(void *k_pages, const int64_t *k_strides, void *v_pages,
+                     const int64_t *v_strides, int64_t layers,
+                     int64_t kv_heads, int64_t head_dim, int32_t *table,
+                     int64_t table_stride, int64_t table_width, int64_t rows,
+                     const int32_t *lengths, int32_t *refs, int64_t pages,
+                     int64_t page_size, int32_t *used, void *workspace,
+                     int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

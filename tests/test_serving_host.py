@@ -1,0 +1,126 @@
+"""The serving operators' refusals, on the CPU: bad calls are turned down before any launch."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tkmi import _lib, ops
+
+S3 = _lib.strides([64, 64, 64])
+S2 = _lib.strides([64, 64])
+S4 = _lib.strides([64, 64, 64, 64])
+
+
+def _window(dtype=1, b=1, h=4, hkv=2, sq=8, sk=8, hd=64, scale=0.1, window=4, sinks=0, q=16, k=16, strides=S3, kv=None,
+            kvs=0):
+    return _lib.load().tk_window_attn(q, S3, k, strides, 16, S3, 16, S3, dtype, b, h, hkv, sq, sk, hd, scale, window,
+                                      sinks, kv, kvs, None)
+
+
+@pytest.mark.parametrize("call,code", [
+    (dict(dtype=0), -1), (dict(dtype=3), -1), (dict(h=3), -1), (dict(sq=9), -1), (dict(window=0), -1),
+    (dict(sinks=-1), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1),
+    (dict(hd=12), -2), (dict(hd=264), -2), (dict(q=None), -1), (dict(k=24), -2), (dict(b=-1), -1),
+    (dict(strides=_lib.strides([64, 64, 60])), -2), (dict(kv=16, kvs=7), -1), (dict(sk=1 << 30), -1),
+    (dict(b=0), 0), (dict(sq=0), 0), (dict(h=0, hkv=0), 0),
+])
+def test_window_attention_refuses(call, code):
+    assert _window(**call) == code
+    assert code == 0 or _lib.load().tk_last_error_string().decode()
+
+
+def _paged(dtype=1, b=2, h=4, hkv=2, hd=64, pages=8, ps=16, table=16, stride=4, width=4, lengths=16, most=64, scale=0.1,
+           window=0, sinks=0, invariant=0, ws=None, size=0, q=16, k=16, strides=S3):
+    return _lib.load().tk_paged_attn(q, S2, k, strides, 16, S3, 16, S2, dtype, b, h, hkv, hd, pages, ps, table, stride,
+                                     width, lengths, most, scale, window, sinks, invariant, ws, size, None)
+
+
+@pytest.mark.parametrize("call,code", [
+    (dict(dtype=0), -1), (dict(h=5), -1), (dict(hd=20), -2), (dict(hd=320), -2), (dict(ps=8), -2), (dict(ps=48), -2),
+    (dict(ps=2048), -2), (dict(stride=3), -1), (dict(table=None), -1), (dict(lengths=None), -1), (dict(scale=-1.0), -1),
+    (dict(window=-1), -1), (dict(sinks=-2), -1), (dict(k=8), -2), (dict(k=None), -1), (dict(pages=-1), -1),
+    (dict(strides=_lib.strides([4, 64, 64])), -2), (dict(most=-1), -1), (dict(width=1 << 26, stride=1 << 26), -1),
+    (dict(most=1 << 20), -1),  # splits its keys and has no workspace
+    (dict(most=1 << 20, ws=8, size=1 << 30), -1), (dict(most=1 << 20, ws=16, size=100), -1),
+    (dict(b=0), 0), (dict(h=0, hkv=0), 0),
+])
+def test_paged_attention_refuses(call, code):
+    assert _paged(**call) == code
+    assert code == 0 or _lib.load().tk_last_error_string().decode()
+
+
+def test_paged_workspace():
+    size = _lib.load().tk_paged_attn_workspace
+    assert size(0, 8, 8, 64, 100000, 0, 0, 0) == 0
+    assert size(1, 8, 8, 64, 16, 0, 0, 0) == 0  # one split writes its results
+    assert size(1, 8, 8, 64, 100000, 0, 0, 0) % (8 * 66 * 4) == 0 and size(1, 8, 8, 64, 100000, 0, 0, 0) > 0
+    assert size(1, 8, 8, 64, 100000, 64, 4, 0) <= size(1, 8, 8, 64, 100000, 0, 0, 0)
+    assert size(1, 8, 3, 64, 16, 0, 0, 0) == -1 and size(1, 8, 8, 36, 16, 0, 0, 0) == -2
+    # batch-invariant splits: their number goes with the length alone
+    assert size(2, 8, 8, 64, 5000, 0, 0, 1) == 2 * size(1, 8, 8, 64, 5000, 0, 0, 1)
+
+
+def test_cache_calls_refuse():
+    lib = _lib.load()
+
+    def append(b=1, n=1, hkv=1, hd=64, pages=4, ps=16, k=16, strides=S3, table=16, lengths=16, width=4, stride=4):
+        return lib.tk_cache_append(k, strides, 16, S3, 16, S3, 16, S3, b, n, hkv, hd, pages, ps, table, stride, width,
+                                   lengths, None, None)
+
+    for call, code in [(dict(hd=12), -2), (dict(ps=24), -2), (dict(k=None), -1), (dict(k=2), -2), (dict(n=-1), -1),
+                       (dict(lengths=None), -1), (dict(table=None), -1), (dict(b=2, stride=3), -1),
+                       (dict(strides=_lib.strides([64, 7, 64])), -2), (dict(n=0), 0), (dict(b=0), 0),
+                       (dict(pages=0), 0)]:
+        assert append(**call) == code, call
+
+    def state(rows=2, width=4, stride=4, table=16, lengths=16, refs=16, pages=8, ps=16):
+        return (table, stride, width, rows, lengths, refs, pages, ps)
+
+    def reserve(new=16, status=16, ws=16, size=1 << 20, **kw):
+        return lib.tk_cache_reserve(*state(**kw), new, status, ws, size, None)
+
+    for call, code in [(dict(new=None), -1), (dict(status=None), -1), (dict(ws=None), -1), (dict(size=39), -1),
+                       (dict(ps=0), -2), (dict(refs=None), -1), (dict(lengths=None), -1), (dict(stride=2), -1),
+                       (dict(rows=-1), -1), (dict(pages=-1), -1)]:
+        assert reserve(**call) == code, call
+
+    def pages_args(k=16, layers=1, hkv=2, hd=64, strides=S4):
+        return (k, strides, 16, S4, layers, hkv, hd)
+
+    def fork(parents=16, children=16, n=1, status=16, ws=16, size=1 << 20, cache=pages_args(), **kw):
+        return lib.tk_cache_fork(*cache, *state(**kw), parents, children, n, status, ws, size, None)
+
+    for call, code in [(dict(parents=None), -1), (dict(n=-1), -1), (dict(status=None), -1), (dict(size=50), -1),
+                       (dict(cache=pages_args(k=None)), -1), (dict(cache=pages_args(k=8)), -2),
+                       (dict(cache=pages_args(hd=4)), -2), (dict(cache=pages_args(layers=-1)), -1),
+                       (dict(cache=pages_args(strides=_lib.strides([1, 64, 64, 64]))), -2),
+                       (dict(cache=pages_args(hkv=65535, hd=256), ps=1024), -1), (dict(width=-1), -1)]:
+        assert fork(**call) == code, call
+    assert lib.tk_cache_free(*state(), None, 1, None) == -1
+    assert lib.tk_cache_free(*state(), 16, -1, None) == -1
+    assert lib.tk_cache_free(*state(), None, 0, None) == 0
+    assert lib.tk_cache_compact(*pages_args(), *state(), None, 16, 1 << 20, None) == -1
+    assert lib.tk_cache_compact(*pages_args(), *state(), 16, 16, 4 * 16, None) == -1
+    assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (2 + 9 + 16)
+
+
+def test_wrappers_refuse_on_the_cpu():
+    half = torch.zeros(1, 2, 4, 64, dtype=torch.float16)
+    table, vec = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.window_attention(half, half, half, 0.1, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.paged_attention(half[:, :, 0], half, half, table, vec, 0.1)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.cache_append(half, half, half, half, table, vec)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.cache_reserve(table, vec, vec, vec, 16)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.cache_free(table, vec, vec, vec, 16)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.cache_fork(half, half, table, vec, vec, vec, vec)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.cache_compact(half, half, table, vec, vec)
+    with pytest.raises(TypeError, match="int32"):
+        ops.cache_reserve(table.long(), vec, vec, vec, 16)

@@ -1,0 +1,306 @@
+// Causal attention over a sliding window of keys and a few first ones (sinks) that stay visible.
+//
+// The query row i of q_len sits at position p = k_len - q_len + i and sees key j when
+//   j <= p  and  (j > p - window  or  j < sinks)  and  key_valid[b, j];
+// a row that sees nothing is 0.  heads / kv_heads query heads share a key head.
+//
+// Bound by the matrix cores (4 head_dim flops per visible pair) and the exponentials beside
+// them; only the 64-key tiles that some row of a workgroup sees are visited: those of the
+// sinks, then those of the window.  A workgroup has 32 rows of one head per wave; K and V tiles
+// go global -> LDS by direct copies one tile ahead, two slots each, one barrier per tile.
+//
+// As in tk_attention.hip a wave computes S^T = K . Q^T (a lane holds one query row's scores, the
+// running maximum is one lane-pair exchange) and O^T = V^T . P^T with the accumulator's keys as
+// the product's k slots and V^T from transposed LDS reads.  The running maximum is raised only
+// when a tile exceeds it by more than 2^8: O and the sums may hold weights up to 256, harmless in
+// fp32 and in 16-bit P, and the rescale of O is skipped on most tiles.
+//
+// Numerics: fp32 scores, maxima, sums, O; P rounded to the inputs' type for the product (half a
+// step: fp16 2^-11, bf16 2^-8 of the weight), the sum taken of the rounded weights, so that they
+// add up to 1.
+#include "tk_attn_tile.hpp"
+#include "tk_elem.hpp"
+
+namespace tk {
+namespace {
+
+struct WindowArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const uint8_t* kv;  // nullable [batch][k_len]
+  int64_t kvs;
+  int64_t qs[3], ks[3], vs[3], os[3];  // elements, {b, h, s}
+  int batch, heads, group, q_len, k_len, hd, window, sinks;
+  int n_qt;
+  float scale_log2;
+};
+
+template <typename T, int DT, int BN, int NW, bool KMASK>
+__device__ __forceinline__ void window_body(const WindowArgs& p) {
+  typedef typename Elem<T>::x8 x8;
+  typedef typename Elem<T>::x4 x4;
+  constexpr int NB = BN / 32;
+  constexpr int RB = DT * 2;
+  constexpr int CPR = RB / 16;
+  constexpr int TILE = BN * RB;
+  constexpr int COPIES = TILE / 1024 / NW;  // per wave, K or V
+  constexpr int RPC = 1024 / RB;
+  constexpr int DB = DT / 32;
+  constexpr int KSTEPS = DT / 16;
+  static_assert(COPIES >= 1 && COPIES * NW * 1024 == TILE, "whole copies per wave");
+  __shared__ __attribute__((aligned(16))) char smem[4 * TILE];  // K, V slots 0; K, V slots 1
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 5;
+
+  // an XCD (block id mod 8) takes neighbouring query tiles of the same heads: they share keys in its L2
+  const int total = p.n_qt * p.batch * p.heads, per = (total + 7) / 8;
+  const int lin = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (lin >= total) return;
+  const int bh = lin / p.n_qt, qt = p.n_qt - 1 - lin % p.n_qt;
+  const int b = bh / p.heads, h = bh % p.heads, kvh = h / p.group;
+
+  const int q0 = qt * (32 * NW);
+  const int shift = p.k_len - p.q_len;
+  const int row = q0 + wave * 32 + (lane & 31);
+  const int pos = shift + row;
+  const int w_lo = shift + q0 + wave * 32, w_hi = w_lo + 31;                    // positions of the wave's rows
+  const int g_hi = min(shift + q0 + 32 * NW - 1, p.k_len - 1);                  // last position of the workgroup's
+  const int lo = max(0, shift + q0 - p.window + 1);                             // first key of any of its windows
+  const int wt = lo / BN;
+  const int st = min((min(p.sinks, lo) + BN - 1) / BN, wt);
+  const int n_kt = st + (g_hi / BN + 1) - wt;
+  auto tile_key = [&](int t) { return (t < st ? t : t - st + wt) * BN; };
+
+  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + kvh * p.ks[1];
+  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + kvh * p.vs[1];
+  const uint8_t* kvb = KMASK ? p.kv + b * p.kvs : nullptr;
+  const uint32_t lds0 = (uint32_t)(size_t)(lds_char*)smem;
+  const int last_chunk = p.hd / 8 - 1;
+
+  // Lane l of copy c fills physical chunk l % CPR of row c * RPC + l / CPR with the logical chunk
+  // that the swizzle keeps there.  Rows past the keys re-read the last one and chunks past head_dim
+  // the last one: their scores are masked, their columns meet zeros of Q or are not stored.
+  auto copy = [&](const T* base, int64_t rs, int k0, uint32_t dst, bool is_v) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int c = wave * COPIES + i;
+      const int r = c * RPC + lane / CPR, phys = lane % CPR;
+      const int chunk = is_v ? phys ^ vswz<RB>(r) : (swz_off<RB>(r, phys) - r * RB) >> 4;
+      dma16(base + (int64_t)min(k0 + r, p.k_len - 1) * rs + min(chunk, last_chunk) * 8, dst + c * 1024);
+    }
+  };
+
+  x8 qf[KSTEPS];
+  {
+    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + (int64_t)min(row, p.q_len - 1) * p.qs[2];
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      const int d = 16 * kk + 8 * g;
+      qf[kk] = x8{};
+      if (d < p.hd) qf[kk] = *reinterpret_cast<const x8*>(qr + d);
+    }
+  }
+  int v_rd[2][DB];  // transposed V reads, as attend_one_tile
+  {
+    const int tq = lane >> 4, ts = lane & 15;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int vr = 8 * r + 4 * (tq >> 1) + (ts >> 2);
+        const int col = 32 * d + 16 * (tq & 1) + 4 * (ts & 3);
+        v_rd[r][d] = vr * RB + (((col >> 3) ^ vswz<RB>(vr)) << 4) + (col & 7) * 2;
+      }
+  }
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float cs = p.scale_log2;
+
+  copy(kb, p.ks[2], tile_key(0), lds0, false);
+  copy(vb, p.vs[2], tile_key(0), lds0 + TILE, true);
+  for (int t = 0; t < n_kt; ++t) {
+    const int k0 = tile_key(t);
+    char* ks_ = smem + (t & 1) * 2 * TILE;
+    char* vs_ = ks_ + TILE;
+    uint64_t bits = ~0ull;
+    if (KMASK) {
+      const int key = k0 + lane;
+      bits = __ballot(lane < BN && key < p.k_len && kvb[min(key, p.k_len - 1)] != 0);
+    }
+    wait_vmcnt<0>();
+    if (KMASK && bits != (BN == 64 ? ~0ull : (1ull << BN) - 1)) {
+      // whatever lies in rows that are not valid times a weight of 0 must be 0
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int c = wave * COPIES + i;
+        if (!((bits >> (c * RPC + lane / CPR)) & 1)) *reinterpret_cast<u32x4*>(vs_ + c * 1024 + lane * 16) = u32x4{};
+      }
+      __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+    }
+    lds_barrier();
+    if (t + 1 < n_kt) {
+      const uint32_t nxt = lds0 + ((t + 1) & 1) * 2 * TILE;
+      copy(kb, p.ks[2], tile_key(t + 1), nxt, false);
+      copy(vb, p.vs[2], tile_key(t + 1), nxt + TILE, true);
+    }
+    // nothing of this tile for any of the wave's rows
+    if (k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
+
+    f32x16 s[NB];
+#pragma unroll
+    for (int kb2 = 0; kb2 < NB; ++kb2)
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        const x8 kf = *reinterpret_cast<const x8*>(ks_ + swz_off<RB>(kb2 * 32 + (lane & 31), 2 * kk + g));
+        s[kb2] = Elem<T>::mfma32(kf, qf[kk], kk == 0 ? f32x16{} : s[kb2]);
+      }
+    const bool whole = k0 + BN - 1 <= w_lo && (k0 > w_hi - p.window || k0 + BN <= p.sinks);
+    if (KMASK || !whole) {
+      const uint64_t kbits = bits >> (4 * g);
+#pragma unroll
+      for (int e = 0; e < 16 * NB; ++e) {
+        const int j = (e >> 4) * 32 + 8 * ((e & 15) >> 2) + (e & 3), key = k0 + j + 4 * g;
+        const bool see = key <= pos && (key > pos - p.window || key < p.sinks) && (!KMASK || ((kbits >> j) & 1));
+        if (!see) s[e >> 4][e & 15] = -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16 * NB; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+    const float m_tile = pair_max(mx) * cs;
+    if (__ballot(m_tile > m_run + 8.f) != 0ull) {
+      const float m_new = fmaxf(m_run, m_tile);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf[2 * NB];
+    float ls = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16 * NB; ++e) {
+      const T pe = (T)__builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], cs, -m_use));
+      pf[e >> 3][e & 7] = pe;
+      ls += (float)pe;
+    }
+    l_run += ls;
+#pragma unroll
+    for (int c = 0; c < 2 * NB * DB; ++c) {
+      const int t16 = c / DB, d = c % DB;
+      const lds_char* base = (const lds_char*)(vs_ + t16 * 16 * RB);
+      const tr_f16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_f16x4*)(base + v_rd[0][d]));
+      const tr_f16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_f16x4*)(base + v_rd[1][d]));
+      const f16x8 vf = __builtin_shufflevector(__builtin_bit_cast(f16x4, lo4), __builtin_bit_cast(f16x4, hi4), 0, 1, 2,
+                                               3, 4, 5, 6, 7);
+      acc[d] = Elem<T>::mfma32(__builtin_bit_cast(x8, vf), pf[t16], acc[d]);
+    }
+  }
+
+  const float l = pair_sum(l_run);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (row < p.q_len) {
+    T* orow = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int dd = d * 32 + 8 * q + 4 * g;
+        if (dd < p.hd)
+          *reinterpret_cast<x4*>(orow + dd) = x4{(T)(acc[d][4 * q] * inv), (T)(acc[d][4 * q + 1] * inv),
+                                                 (T)(acc[d][4 * q + 2] * inv), (T)(acc[d][4 * q + 3] * inv)};
+      }
+  }
+}
+
+template <typename T, int DT, int BN, int NW, bool KMASK>
+__global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_attn_kernel(WindowArgs p) {
+  window_body<T, DT, BN, NW, KMASK>(p);
+}
+
+template <typename T, int DT, int BN>
+int launch_window(WindowArgs p, hipStream_t st) {
+  constexpr int NW = 4;
+  p.n_qt = (p.q_len + 32 * NW - 1) / (32 * NW);
+  const int64_t total = (int64_t)p.n_qt * p.batch * p.heads;
+  TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "tk_window_attn: too many workgroups");
+  const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
+  if (p.kv) hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, true>), g, blk, 0, st, p);
+  else hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, false>), g, blk, 0, st, p);
+  return check_launch("tk_window_attn");
+}
+
+template <typename T>
+int dispatch_window(const WindowArgs& p, hipStream_t st) {
+  if (p.hd <= 32) return launch_window<T, 32, 64>(p, st);
+  if (p.hd <= 64) return launch_window<T, 64, 64>(p, st);
+  if (p.hd <= 128) return launch_window<T, 128, 64>(p, st);
+  return launch_window<T, 256, 32>(p, st);
+}
+
+}  // namespace
+}  // namespace tk
+
+using namespace tk;
+
+extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                              const void* v, const int64_t* v_strides, void* out, const int64_t* o_strides, int dtype,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t k_len,
+                              int64_t head_dim, float scale, int64_t window, int64_t sinks, const uint8_t* key_valid,
+                              int64_t key_valid_stride, void* stream) {
+  const char* fn = "tk_window_attn";
+  TK_REQUIRE(dtype == TK_F16 || dtype == TK_BF16, TK_ERR_ARG, "%s: dtype %d is not TK_F16 or TK_BF16", fn, dtype);
+  TK_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 0 && q_len >= 0 && head_dim >= 0 && sinks >= 0 &&
+                 batch < (1ll << 31) && heads < (1ll << 31) && kv_heads < (1ll << 31),
+             TK_ERR_ARG, "%s: size out of range", fn);
+  TK_REQUIRE(q_len <= k_len && k_len < (1ll << 30), TK_ERR_ARG, "%s: q_len=%lld, k_len=%lld: at most k_len queries", fn,
+             (long long)q_len, (long long)k_len);
+  TK_REQUIRE(window >= 1, TK_ERR_ARG, "%s: window=%lld < 1", fn, (long long)window);
+  TK_REQUIRE(scale > 0.f && scale <= 3.0e38f, TK_ERR_ARG, "%s: scale must be positive and finite", fn);
+  TK_REQUIRE(kv_heads == 0 ? heads == 0 : heads % kv_heads == 0, TK_ERR_ARG,
+             "%s: heads=%lld is no multiple of kv_heads=%lld", fn, (long long)heads, (long long)kv_heads);
+  TK_REQUIRE(head_dim <= 256 && head_dim % 8 == 0, TK_ERR_UNSUPPORTED,
+             "%s: head_dim=%lld is no multiple of 8 up to 256", fn, (long long)head_dim);
+  if (batch == 0 || heads == 0 || q_len == 0 || head_dim == 0) return TK_OK;
+  TK_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides && o_strides, TK_ERR_ARG, "%s: null pointer", fn);
+  TK_REQUIRE(key_valid == nullptr || key_valid_stride >= k_len, TK_ERR_ARG, "%s: key_valid_stride=%lld < k_len", fn,
+             (long long)key_valid_stride);
+  auto al = [](const void* ptr, uintptr_t a) { return ((uintptr_t)ptr % a) == 0; };
+  bool rows = al(q, 16) && al(k, 16) && al(v, 16) && al(out, 8);
+  WindowArgs p{};
+  for (int i = 0; i < 3; ++i) {
+    rows = rows && q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
+    p.qs[i] = q_strides[i];
+    p.ks[i] = k_strides[i];
+    p.vs[i] = v_strides[i];
+    p.os[i] = o_strides[i];
+  }
+  TK_REQUIRE(rows, TK_ERR_UNSUPPORTED, "%s: rows of q, k, v must be 16-byte aligned, of out 8-byte", fn);
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = out;
+  p.kv = key_valid;
+  p.kvs = key_valid_stride;
+  p.batch = (int)batch;
+  p.heads = (int)heads;
+  p.group = (int)(heads / kv_heads);
+  p.q_len = (int)q_len;
+  p.k_len = (int)k_len;
+  p.hd = (int)head_dim;
+  // past every key both change nothing; kept small enough for sums of positions
+  p.window = (int)(window < k_len ? window : k_len);
+  p.sinks = (int)(sinks < k_len ? sinks : k_len);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return dtype == TK_F16 ? dispatch_window<f16>(p, as_stream(stream)) : dispatch_window<bf16>(p, as_stream(stream));
+}

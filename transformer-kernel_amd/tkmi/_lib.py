@@ -13,10 +13,10 @@ import threading
 from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_void_p
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libtkmi.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 TK_OK, TK_ERR_ARG, TK_ERR_UNSUPPORTED, TK_ERR_HIP = 0, -1, -2, -3
-TK_F32, TK_F16 = 0, 1
+TK_F32, TK_F16, TK_BF16 = 0, 1, 2
 TK_EPI_BIAS, TK_EPI_BIAS_GELU, TK_EPI_BIAS_RESID = 0, 1, 2
 TK_ROWS_KEEP_RESID, TK_ROWS_ZERO, TK_ROWS_ZERO_ALL = 1, 2, 3
 
@@ -24,6 +24,10 @@ TK_FWD_FUSED_NORM, TK_FWD_QKV_ATTENTION, TK_FWD_BATCH_INVARIANT = 1, 2, 4
 TK_FWD_IO_F16, TK_FWD_IO_BF16 = 8, 16
 
 _I64_3 = c_int64 * 3
+_STRIDES = POINTER(c_int64)
+# table, its row stride and width, rows, lengths, refs, pages, page_size (the cache calls)
+_TABLE = [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64]
+_PAGES = [c_void_p, _STRIDES, c_void_p, _STRIDES, c_int64, c_int64, c_int64]  # k, v, layers, kv_heads, head_dim
 
 
 class Layer(ctypes.Structure):
@@ -115,6 +119,27 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64,
          c_void_p],
     ),
+    "tk_window_attn": (
+        c_int,
+        [c_void_p, _STRIDES] * 4 + [c_int] + [c_int64] * 6 + [c_float, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "tk_paged_attn_workspace": (c_int64, [c_int64] * 7 + [c_int]),
+    "tk_paged_attn": (
+        c_int,
+        [c_void_p, _STRIDES] * 4 + [c_int] + [c_int64] * 6
+        + [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_float, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p],
+    ),
+    "tk_cache_workspace": (c_int64, [c_int64] * 3),
+    "tk_cache_append": (
+        c_int,
+        [c_void_p, _STRIDES] * 4 + [c_int64] * 6 + [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    "tk_cache_reserve": (c_int, _TABLE + [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "tk_cache_fork": (
+        c_int, _PAGES + _TABLE + [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
+    ),
+    "tk_cache_free": (c_int, _TABLE + [c_void_p, c_int64, c_void_p]),
+    "tk_cache_compact": (c_int, _PAGES + _TABLE + [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 for _name in ("tk_gemm", "tk_gemm_bias_add_ln", "tk_flash_attn_fwd"):
     SIGNATURES[_name + "_invariant"] = SIGNATURES[_name]
@@ -176,3 +201,7 @@ def call(name: str, *args) -> None:
 
 def strides3(values) -> "ctypes.Array":
     return _I64_3(*[int(v) for v in values])
+
+
+def strides(values) -> "ctypes.Array":
+    return (c_int64 * len(values))(*values)

@@ -4,7 +4,10 @@ Names and argument meanings follow the reference's kernel wrappers:
   ``can_fuse``, ``ln_fwd``, ``add_ln_fwd``      -- src/fused_kernels.py:62-64,164-238
   ``attention_supported``, ``flash_attention``  -- src/kernels.py:96-103,250-294
 plus the GEMM entry points that replace ``F.linear`` (+GELU / +residual /
-+residual+LayerNorm) and the standalone masked softmax.
++residual+LayerNorm), the standalone masked softmax, and for serving a causal
+stack token by token: ``window_attention``, ``paged_attention`` and the
+``cache_*`` operators of the paged key/value cache that it reads (no
+counterparts in the reference).
 
 Every wrapper launches on torch's current HIP stream and allocates its
 outputs with ``torch.empty`` (the caching allocator).  There is no CPU or
@@ -21,7 +24,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import (TK_EPI_BIAS, TK_EPI_BIAS_GELU, TK_EPI_BIAS_RESID, TK_F16, TK_F32, TK_ROWS_KEEP_RESID,
+from ._lib import (TK_BF16, TK_EPI_BIAS, TK_EPI_BIAS_GELU, TK_EPI_BIAS_RESID, TK_F16, TK_F32, TK_ROWS_KEEP_RESID,
                    TK_ROWS_ZERO, TK_ROWS_ZERO_ALL)
 
 MAX_FUSED_SIZE = 8192  # longest LayerNorm row (src/fused_kernels.py:59)
@@ -436,3 +439,277 @@ def masked_softmax(scores, causal: bool, key_len=None, heads_per_batch: int = 1)
         _stream(sc),
     )
     return probs
+
+
+# --------------------------------------------------------------------------- #
+# Serving: window attention, a paged key/value cache, one new token over it
+# --------------------------------------------------------------------------- #
+
+_HALF_CODE = {torch.float16: TK_F16, torch.bfloat16: TK_BF16}
+
+
+def _launch_on(device: torch.device, name: str, fn: str, *args) -> None:
+    """A launch with the tensors' device current, on its current stream."""
+    with torch.cuda.device(device):
+        _launch(name, fn, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _strides_of(t: torch.Tensor, dims) -> "ctypes.Array":
+    """Element strides of ``dims``; those of a dimension of one entry are never used."""
+    return _lib.strides([t.stride(i) if t.shape[i] > 1 else 0 for i in dims])
+
+
+def _check_half(what: str, **tensors: torch.Tensor) -> int:
+    """One 16-bit dtype, one device, contiguous last dimensions; returns the dtype's code."""
+    first = next(iter(tensors.values()))
+    _require_cuda(*tensors.values())
+    for name, t in tensors.items():
+        if t.dtype not in _HALF_CODE or t.dtype != first.dtype:
+            raise TypeError(f"{what}: {name} is {t.dtype}; expected one of float16 and bfloat16 for all")
+        if t.device != first.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, not {first.device}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{what}: {name} needs a contiguous head_dim")
+    return _HALF_CODE[first.dtype]
+
+
+def _check_int32(what: str, device, entries: Optional[int] = None, **tensors) -> None:
+    """Contiguous int32 vectors on ``device``, of ``entries`` entries if given."""
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise TypeError(f"{what}: {name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
+        if entries is not None and t.shape[0] != entries:
+            raise ValueError(f"{what}: {name} must have {entries} entries, got {t.shape[0]}")
+        _require_cuda(t)
+        if t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, not {device}")
+
+
+def _check_table(what: str, table: torch.Tensor, lengths: torch.Tensor) -> tuple:
+    """table [rows, entries] and lengths [rows]; returns (pointer, row stride, entries)."""
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise TypeError(f"{what}: table must be int32 [rows, entries] with contiguous rows, got {table.dtype} "
+                        f"{tuple(table.shape)}")
+    _require_cuda(table)
+    _check_int32(what, table.device, table.shape[0], lengths=lengths)
+    stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    return table.data_ptr(), stride, table.shape[1]
+
+
+def _state_args(what: str, table, lengths, refs, page_size: int) -> tuple:
+    """The table arguments of the cache's bookkeeping (tkmi.h)."""
+    ptr, stride, width = _check_table(what, table, lengths)
+    _check_int32(what, table.device, refs=refs)
+    return (ptr, stride, width, table.shape[0], lengths.data_ptr(), refs.data_ptr(), refs.shape[0], int(page_size))
+
+
+def _cache_args(what: str, k_pages, v_pages, refs) -> tuple:
+    """Pages [layers, pages, kv_heads, page_size, head_dim], or of one layer without the first dimension."""
+    _check_half(what, k_pages=k_pages, v_pages=v_pages)
+    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+        raise ValueError(f"{what}: k_pages and v_pages must share one shape [layers, pages, kv_heads, page_size, "
+                         f"head_dim], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    k = k_pages if k_pages.dim() == 5 else k_pages[None]
+    v = v_pages if v_pages.dim() == 5 else v_pages[None]
+    if k.device != refs.device or k.shape[1] != refs.shape[0]:
+        raise ValueError(f"{what}: refs must have one entry per page ({k.shape[1]}) on {k.device}")
+    return (k.data_ptr(), _strides_of(k, range(4)), v.data_ptr(), _strides_of(v, range(4)), k.shape[0], k.shape[2],
+            k.shape[4])
+
+
+def _cache_workspace(device, rows: int, pages: int, n: int = 0) -> torch.Tensor:
+    size = _lib.load().tk_cache_workspace(rows, pages, n)
+    if size < 0:
+        raise _lib.TkError("tk_cache_workspace", size, _lib.load().tk_last_error_string().decode())
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=None, key_valid=None):
+    """Causal attention over the last ``window`` keys and the first ``sinks``; returns ``[B, Sq, H*hd]``.
+
+    q is ``[B, H, Sq, hd]``, k and v ``[B, Hkv, Sk, hd]`` with ``Sq <= Sk`` and ``H`` a
+    multiple of ``Hkv`` (head h reads key head ``h // (H // Hkv)``), float16 or bfloat16,
+    strided in the first three dims; head_dim a multiple of 8 up to 256, rows 16-byte
+    aligned.  The queries are the last Sq of Sk positions (a chunk of a prompt behind its
+    cached keys): the one at position p sees key j when ``j <= p`` and ``j > p - window``
+    or ``j < sinks``.  ``key_valid`` (optional ``[B, Sk]`` bool): other keys are not seen,
+    whatever they hold; at valid ones K and V must be finite.  A query that sees nothing
+    gets zeros (``flash_attention``: NaN).  ``window >= Sk`` is plain causal attention.
+    A sequence's bits do not depend on the batch.
+    """
+    what = "window_attention"
+    code = _check_half(what, q=q, k=k, v=v)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{what}: q [B, H, Sq, hd] and k, v [B, Hkv, Sk, hd] expected, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    b, h, sq, hd = q.shape
+    hkv, sk = k.shape[1], k.shape[2]
+    if out is None:
+        out = torch.empty((b, sq, h * hd), dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (b, sq, h * hd):
+        raise ValueError(f"{what}: out must be [B, Sq, H*hd] = {(b, sq, h * hd)}, got {tuple(out.shape)}")
+    _check_half(what, q=q, out=out)
+    kv = None
+    if key_valid is not None:
+        if tuple(key_valid.shape) != (b, sk):
+            raise ValueError(f"{what}: key_valid must be [B, Sk] = {(b, sk)}, got {tuple(key_valid.shape)}")
+        kv = _row_mask(key_valid, b * sk)
+        if kv.device != q.device:
+            raise ValueError(f"{what}: key_valid is on {kv.device}, not {q.device}")
+    o_strides = _lib.strides([out.stride(0) if b > 1 else 0, hd if h > 1 else 0, out.stride(1) if sq > 1 else 0])
+    _launch_on(
+        q.device, "window_attn", "tk_window_attn", q.data_ptr(), _strides_of(q, range(3)), k.data_ptr(),
+        _strides_of(k, range(3)), v.data_ptr(), _strides_of(v, range(3)), out.data_ptr(), o_strides, code, b, h, hkv,
+        sq, sk, hd, float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk,
+    )
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: int = 0, sinks: int = 0,
+                    max_length: Optional[int] = None, out=None, batch_invariant: bool = False):
+    """Attention of each sequence's newest token over its pages; returns ``[B, H*hd]``.
+
+    q is ``[B, H, hd]`` (the token at position ``lengths[b] - 1``, whose own key is in the
+    cache already), k_pages and v_pages one layer's ``[pages, Hkv, page_size, hd]``, table
+    ``[B, entries]`` int32 and lengths ``[B]`` int32 (``cache_append`` has the layout).
+    ``window`` (0: every key) and ``sinks`` as in ``window_attention``; the pages of keys
+    outside of both are not read and may be -1.  Keys whose table entry is no page of the
+    cache are not seen; a sequence that sees nothing gets zeros.  ``max_length`` (default:
+    the table's) says how long sequences are expected to be: it sizes the split of the keys
+    over workgroups and changes no result beyond rounding.  ``batch_invariant``: a
+    sequence's bits do not depend on the batch or ``max_length``.
+    """
+    what = "paged_attention"
+    code = _check_half(what, q=q, k_pages=k_pages, v_pages=v_pages)
+    if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or q.shape[2] != k_pages.shape[3]:
+        raise ValueError(f"{what}: q [B, H, hd] and pages [pages, Hkv, page_size, hd] expected, got {tuple(q.shape)}, "
+                         f"{tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+    b, h, hd = q.shape
+    pages, hkv, page_size, _ = k_pages.shape
+    ptr, stride, width = _check_table(what, table, lengths)
+    if table.shape[0] != b or table.device != q.device:
+        raise ValueError(f"{what}: table must have a row per sequence ({b}) on {q.device}")
+    if max_length is None or batch_invariant:
+        max_length = width * page_size
+    if out is None:
+        out = torch.empty((b, h * hd), dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (b, h * hd):
+        raise ValueError(f"{what}: out must be [B, H*hd] = {(b, h * hd)}, got {tuple(out.shape)}")
+    _check_half(what, q=q, out=out)
+    invariant = int(bool(batch_invariant))
+    size = _lib.load().tk_paged_attn_workspace(b, h, hkv, hd, int(max_length), int(window), int(sinks), invariant)
+    if size < 0:
+        raise _lib.TkError("tk_paged_attn_workspace", size, _lib.load().tk_last_error_string().decode())
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    o_strides = _lib.strides([out.stride(0) if b > 1 else 0, hd])
+    _launch_on(
+        q.device, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_of(q, range(2)), k_pages.data_ptr(),
+        _strides_of(k_pages, range(3)), v_pages.data_ptr(), _strides_of(v_pages, range(3)), out.data_ptr(), o_strides,
+        code, b, h, hkv, hd, pages, page_size, ptr, stride, width, lengths.data_ptr(), int(max_length), float(scale),
+        int(window), int(sinks), invariant, ws.data_ptr() if ws is not None else None, size,
+    )
+    return out
+
+
+def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
+    """Writes the newest tokens' keys and values into the pages of one layer.
+
+    k and v are ``[B, n, Hkv, hd]`` (views of a fused projection's output, for instance);
+    k_pages and v_pages ``[pages, Hkv, page_size, hd]`` with page_size a power of two from
+    16 to 1024.  Sequence b has lengths[b] tokens, these included (``cache_reserve`` comes
+    first); token j is row ``j % page_size`` of page ``table[b, j // page_size]``.  Row i of
+    the ``new[b]`` (int32 ``[B]``; default and at most n) goes to position
+    ``lengths[b] - new[b] + i``.  Positions that have no page are left out.
+    """
+    what = "cache_append"
+    _check_half(what, k=k, v=v, k_pages=k_pages, v_pages=v_pages)
+    if k.dim() != 4 or k.shape != v.shape or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
+            k.shape[2:] != (k_pages.shape[1], k_pages.shape[3]):
+        raise ValueError(f"{what}: k, v [B, n, Hkv, hd] and pages [pages, Hkv, page_size, hd] expected, got "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+    b, n, hkv, hd = k.shape
+    pages, _, page_size, _ = k_pages.shape
+    ptr, stride, width = _check_table(what, table, lengths)
+    if table.shape[0] != b or table.device != k.device:
+        raise ValueError(f"{what}: table must have a row per sequence ({b}) on {k.device}")
+    if new is not None:
+        _check_int32(what, k.device, b, new=new)
+    _launch_on(
+        k.device, "cache_append", "tk_cache_append", k.data_ptr(), _strides_of(k, range(3)), v.data_ptr(),
+        _strides_of(v, range(3)), k_pages.data_ptr(), _strides_of(k_pages, range(3)), v_pages.data_ptr(),
+        _strides_of(v_pages, range(3)), b, n, hkv, hd, pages, page_size, ptr, stride, width, lengths.data_ptr(),
+        new.data_ptr() if new is not None else None,
+    )
+
+
+def cache_reserve(table, lengths, refs, new, page_size: int):
+    """Grows every sequence by ``new[b] >= 0`` tokens (int32 ``[rows]``), with the pages that this needs.
+
+    table ``[rows, entries]``, lengths ``[rows]`` and refs ``[pages]`` (how many sequences
+    hold a page; it is free at ``refs <= 0``) are int32 and updated in place; the lowest
+    free pages are taken, row by row.  Returns an int32 tensor of one entry on the device:
+    0 when done; otherwise nothing has changed, and it holds the number of pages that were
+    missing, or -1 for a row that would outgrow the table (or a negative length or count).
+    Decided on the device: a captured graph reserves anew at every replay.
+    """
+    what = "cache_reserve"
+    state = _state_args(what, table, lengths, refs, page_size)
+    _check_int32(what, table.device, table.shape[0], new=new)
+    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0])
+    status = torch.empty(1, dtype=torch.int32, device=table.device)
+    _launch_on(table.device, "cache_reserve", "tk_cache_reserve", *state, new.data_ptr(), status.data_ptr(),
+               ws.data_ptr(), ws.numel())
+    return status
+
+
+def cache_fork(k_pages, v_pages, table, lengths, refs, parents, children):
+    """Makes row ``children[i]`` a copy of sequence ``parents[i]`` (int32 vectors of one length).
+
+    Whole pages are shared (their refs grow by one); the rows of a page that is only begun
+    are copied, in every layer, into a free page, so that both go on writing their own.
+    k_pages and v_pages are ``[layers, pages, Hkv, page_size, hd]`` (or one layer's).  A
+    parent may have several children; a child must be an empty row, named once.  Parents
+    count as they were before the call.  Returns the status as ``cache_reserve`` does: 0,
+    or nothing has changed and it is the number of missing pages, or -1 for a row that is
+    not in the table, a child that is not empty or that is named twice.
+    """
+    what = "cache_fork"
+    cache = _cache_args(what, k_pages, v_pages, refs)
+    state = _state_args(what, table, lengths, refs, k_pages.shape[-2])
+    _check_int32(what, table.device, parents=parents)
+    _check_int32(what, table.device, parents.shape[0], children=children)
+    n = parents.shape[0]
+    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0], n)
+    status = torch.empty(1, dtype=torch.int32, device=table.device)
+    _launch_on(table.device, "cache_fork", "tk_cache_fork", *cache, *state, parents.data_ptr(), children.data_ptr(), n,
+               status.data_ptr(), ws.data_ptr(), ws.numel())
+    return status
+
+
+def cache_free(table, lengths, refs, rows, page_size: int) -> None:
+    """Ends the sequences of ``rows`` (int32): their pages' refs drop, their entries become -1, their lengths 0.
+
+    Rows that are not in the table are passed over; one that is listed twice is freed once.
+    """
+    what = "cache_free"
+    state = _state_args(what, table, lengths, refs, page_size)
+    _check_int32(what, table.device, rows=rows)
+    _launch_on(table.device, "cache_free", "tk_cache_free", *state, rows.data_ptr(), rows.shape[0])
+
+
+def cache_compact(k_pages, v_pages, table, lengths, refs):
+    """Moves the live pages to the front of the cache, as few as possible; returns their number.
+
+    With ``used`` live pages, the i-th live page of those with id >= used moves into the
+    i-th free one below, in every layer of ``[layers, pages, Hkv, page_size, hd]``; table
+    and refs follow.  Pages ``[used, pages)`` are free afterwards.  The int32 tensor of one
+    entry stays on the device.
+    """
+    what = "cache_compact"
+    cache = _cache_args(what, k_pages, v_pages, refs)
+    state = _state_args(what, table, lengths, refs, k_pages.shape[-2])
+    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0])
+    used = torch.empty(1, dtype=torch.int32, device=table.device)
+    _launch_on(table.device, "cache_compact", "tk_cache_compact", *cache, *state, used.data_ptr(), ws.data_ptr(),
+               ws.numel())
+    return used
