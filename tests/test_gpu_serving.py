@@ -5,6 +5,8 @@ Tolerances are those of serving_reference.tolerance, derived from the operands' 
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -96,6 +98,21 @@ def test_window_scores_that_rise_and_fall():
     for sign in (1, -1):
         _check_window(q, (k.float() + sign * ramp).half(), v, 100, 4)
         _check_window(q.abs(), (-(k.float().abs()) * 3 + sign * ramp).half(), v, 100, 4)
+
+
+@pytest.mark.parametrize("low", [2.0 ** -15, 2.0 ** -18, 2.0 ** -22])
+def test_window_many_small_weights(low):
+    """One key of weight 1 and 3000 of a weight below fp16's normal range that together matter."""
+    s, hd = 3001, 64
+    q = torch.zeros(1, 1, s, hd, dtype=F16)
+    q[..., 0] = 1.0
+    k = torch.zeros(1, 1, s, hd, dtype=F16)
+    k[:, :, 1:, 0] = math.log(low)
+    v = seeded(1, 1, s, hd, dtype=F16, seed=18).abs() + 1
+    v[:, :, 0] = 0
+    for dtype in (F16, BF16):
+        _check_window(q.to(dtype), k.to(dtype), v.to(dtype), s, 0, scale=1.0)
+        _check_window(q.to(dtype)[:, :, -2:], k.to(dtype), v.to(dtype), 2000, 1, scale=1.0)
 
 
 def test_window_views_out_and_neighbours():

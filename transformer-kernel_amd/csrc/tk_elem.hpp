@@ -5,6 +5,7 @@
 namespace tk {
 
 typedef __bf16 bf16;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -23,6 +24,13 @@ struct Elem<f16> {
   static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  // c + the sum of a's values, two to an instruction
+  static __device__ __forceinline__ float sum8(x8 a, float c) {
+    const hf16x2 one = {(__fp16)1.f, (__fp16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2(__builtin_bit_cast(hf16x2, f16x2{a[i], a[i + 1]}), one, c, false);
+    return c;
+  }
 };
 
 template <>
@@ -34,6 +42,12 @@ struct Elem<bf16> {
   }
   static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum8(x8 a, float c) {
+    const bf16x2 one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[i], a[i + 1]}, one, c, false);
+    return c;
   }
 };
 

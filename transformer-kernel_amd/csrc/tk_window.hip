@@ -84,13 +84,30 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
   // Lane l of copy c fills physical chunk l % CPR of row c * RPC + l / CPR with the logical chunk
   // that the swizzle keeps there.  Rows past the keys re-read the last one and chunks past head_dim
   // the last one: their scores are masked, their columns meet zeros of Q or are not stored.
-  auto copy = [&](const T* base, int64_t rs, int k0, uint32_t dst, bool is_v) {
+  // A lane's row and chunk never change: their address is kept, and only the tile's is added (a
+  // 64-bit product per copy and lane was a fifth of the loop's vector instructions).
+  const T *kp[COPIES], *vp[COPIES];
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int c = wave * COPIES + i;
-      const int r = c * RPC + lane / CPR, phys = lane % CPR;
-      const int chunk = is_v ? phys ^ vswz<RB>(r) : (swz_off<RB>(r, phys) - r * RB) >> 4;
-      dma16(base + (int64_t)min(k0 + r, p.k_len - 1) * rs + min(chunk, last_chunk) * 8, dst + c * 1024);
+  for (int i = 0; i < COPIES; ++i) {
+    const int r = (wave * COPIES + i) * RPC + lane / CPR, phys = lane % CPR;
+    kp[i] = kb + r * p.ks[2] + min((swz_off<RB>(r, phys) - r * RB) >> 4, last_chunk) * 8;
+    vp[i] = vb + r * p.vs[2] + min(phys ^ vswz<RB>(r), last_chunk) * 8;
+  }
+  auto copy = [&](int t, uint32_t dst) {
+    const int k0 = tile_key(t);
+    const int64_t ko = k0 * p.ks[2], vo = k0 * p.vs[2];
+    if (k0 + BN <= p.k_len) {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) dma16(kp[i] + ko, dst + (wave * COPIES + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) dma16(vp[i] + vo, dst + TILE + (wave * COPIES + i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int r = (wave * COPIES + i) * RPC + lane / CPR, back = max(k0 + r - (p.k_len - 1), 0);
+        dma16(kp[i] + ko - back * p.ks[2], dst + (wave * COPIES + i) * 1024);
+        dma16(vp[i] + vo - back * p.vs[2], dst + TILE + (wave * COPIES + i) * 1024);
+      }
     }
   };
 
@@ -123,8 +140,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
   float m_run = -INFINITY, l_run = 0.f;
   const float cs = p.scale_log2;
 
-  copy(kb, p.ks[2], tile_key(0), lds0, false);
-  copy(vb, p.vs[2], tile_key(0), lds0 + TILE, true);
+  copy(0, lds0);
   for (int t = 0; t < n_kt; ++t) {
     const int k0 = tile_key(t);
     char* ks_ = smem + (t & 1) * 2 * TILE;
@@ -145,19 +161,15 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
       __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
     }
     lds_barrier();
-    if (t + 1 < n_kt) {
-      const uint32_t nxt = lds0 + ((t + 1) & 1) * 2 * TILE;
-      copy(kb, p.ks[2], tile_key(t + 1), nxt, false);
-      copy(vb, p.vs[2], tile_key(t + 1), nxt + TILE, true);
-    }
+    if (t + 1 < n_kt) copy(t + 1, lds0 + ((t + 1) & 1) * 2 * TILE);
     // nothing of this tile for any of the wave's rows
     if (k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
 
     f32x16 s[NB];
 #pragma unroll
-    for (int kb2 = 0; kb2 < NB; ++kb2)
+    for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < KSTEPS; ++kk) {
+      for (int kb2 = 0; kb2 < NB; ++kb2) {
         const x8 kf = *reinterpret_cast<const x8*>(ks_ + swz_off<RB>(kb2 * 32 + (lane & 31), 2 * kk + g));
         s[kb2] = Elem<T>::mfma32(kf, qf[kk], kk == 0 ? f32x16{} : s[kb2]);
       }
@@ -187,14 +199,11 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
     x8 pf[2 * NB];
-    float ls = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16 * NB; ++e) {
-      const T pe = (T)__builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], cs, -m_use));
-      pf[e >> 3][e & 7] = pe;
-      ls += (float)pe;
-    }
-    l_run += ls;
+    for (int e = 0; e < 16 * NB; ++e)
+      pf[e >> 3][e & 7] = (T)__builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], cs, -m_use));
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) l_run = Elem<T>::sum8(pf[i], l_run);
 #pragma unroll
     for (int c = 0; c < 2 * NB * DB; ++c) {
       const int t16 = c / DB, d = c % DB;

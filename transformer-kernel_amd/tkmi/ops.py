@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -447,81 +448,109 @@ def masked_softmax(scores, causal: bool, key_len=None, heads_per_batch: int = 1)
 
 _HALF_CODE = {torch.float16: TK_F16, torch.bfloat16: TK_BF16}
 
-
-def _launch_on(device: torch.device, name: str, fn: str, *args) -> None:
-    """A launch with the tensors' device current, on its current stream."""
-    with torch.cuda.device(device):
-        _launch(name, fn, *args, torch.cuda.current_stream(device).cuda_stream)
+# A decode step is a few calls of some microseconds per layer, so what a call does on the host is
+# kept short: one pass over the tensors that are all right, and descriptions of what is wrong
+# only where something is.
 
 
-def _strides_of(t: torch.Tensor, dims) -> "ctypes.Array":
-    """Element strides of ``dims``; those of a dimension of one entry are never used."""
-    return _lib.strides([t.stride(i) if t.shape[i] > 1 else 0 for i in dims])
+def _launch_on(index: int, name: str, fn: str, *args) -> None:
+    """A launch on the current stream of device ``index``, with that device current."""
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if index == torch.cuda.current_device():
+        _launch(name, fn, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            _launch(name, fn, *args, stream)
 
 
-def _check_half(what: str, **tensors: torch.Tensor) -> int:
-    """One 16-bit dtype, one device, contiguous last dimensions; returns the dtype's code."""
-    first = next(iter(tensors.values()))
-    _require_cuda(*tensors.values())
-    for name, t in tensors.items():
-        if t.dtype not in _HALF_CODE or t.dtype != first.dtype:
+@functools.lru_cache(maxsize=4096)
+def _strides_array(shape, stride, dims: int) -> "ctypes.Array":
+    """The strides of the first ``dims`` dimensions (read only); those of one entry are never used."""
+    return _lib.strides([st if n > 1 else 0 for n, st in zip(shape[:dims], stride)])
+
+
+def _strides_of(t: torch.Tensor, dims: int) -> "ctypes.Array":
+    return _strides_array(t.shape, t.stride(), dims)
+
+
+def _check_half(what: str, names: str, *tensors: torch.Tensor) -> int:
+    """One 16-bit dtype, one device, contiguous last dimensions; returns the device's index."""
+    dtype, index = tensors[0].dtype, tensors[0].get_device()
+    if index >= 0 and dtype in _HALF_CODE:
+        for t in tensors:
+            if t.dtype is not dtype or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
+                break
+        else:
+            return index
+    _require_cuda(*tensors)
+    for name, t in zip(names.split(), tensors):
+        if t.dtype not in _HALF_CODE or t.dtype != dtype:
             raise TypeError(f"{what}: {name} is {t.dtype}; expected one of float16 and bfloat16 for all")
-        if t.device != first.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, not {first.device}")
+        if t.get_device() != index:
+            raise ValueError(f"{what}: {name} is on {t.device}, not {tensors[0].device}")
         if t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{what}: {name} needs a contiguous head_dim")
-    return _HALF_CODE[first.dtype]
+    raise AssertionError("unreachable")
 
 
-def _check_int32(what: str, device, entries: Optional[int] = None, **tensors) -> None:
-    """Contiguous int32 vectors on ``device``, of ``entries`` entries if given."""
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise TypeError(f"{what}: {name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-        if entries is not None and t.shape[0] != entries:
-            raise ValueError(f"{what}: {name} must have {entries} entries, got {t.shape[0]}")
+def _check_int32(what: str, name: str, t: torch.Tensor, index: int, entries: Optional[int] = None) -> int:
+    """A contiguous int32 vector on device ``index``, of ``entries`` entries if given; returns its address."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{what}: {name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
+    if entries is not None and t.shape[0] != entries:
+        raise ValueError(f"{what}: {name} must have {entries} entries, got {t.shape[0]}")
+    if t.get_device() != index:
         _require_cuda(t)
-        if t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, not {device}")
+        raise ValueError(f"{what}: {name} is on {t.device}, not cuda:{index}")
+    return t.data_ptr()
 
 
-def _check_table(what: str, table: torch.Tensor, lengths: torch.Tensor) -> tuple:
-    """table [rows, entries] and lengths [rows]; returns (pointer, row stride, entries)."""
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+def _check_table(what: str, table: torch.Tensor, index: int) -> tuple:
+    """table [rows, entries] on device ``index``; returns (pointer, row stride, entries, rows)."""
+    if table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
         raise TypeError(f"{what}: table must be int32 [rows, entries] with contiguous rows, got {table.dtype} "
                         f"{tuple(table.shape)}")
-    _require_cuda(table)
-    _check_int32(what, table.device, table.shape[0], lengths=lengths)
-    stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-    return table.data_ptr(), stride, table.shape[1]
+    if table.get_device() != index or index < 0:
+        _require_cuda(table)
+        raise ValueError(f"{what}: table is on {table.device}, not cuda:{index}")
+    rows, width = table.shape
+    return table.data_ptr(), table.stride(0) if rows > 1 else width, width, rows
 
 
 def _state_args(what: str, table, lengths, refs, page_size: int) -> tuple:
-    """The table arguments of the cache's bookkeeping (tkmi.h)."""
-    ptr, stride, width = _check_table(what, table, lengths)
-    _check_int32(what, table.device, refs=refs)
-    return (ptr, stride, width, table.shape[0], lengths.data_ptr(), refs.data_ptr(), refs.shape[0], int(page_size))
+    """The table arguments of the cache's bookkeeping (tkmi.h); the fourth is the number of rows."""
+    index = table.get_device()
+    state = _check_table(what, table, index)
+    return (*state, _check_int32(what, "lengths", lengths, index, state[3]), _check_int32(what, "refs", refs, index),
+            refs.shape[0], int(page_size))
 
 
 def _cache_args(what: str, k_pages, v_pages, refs) -> tuple:
     """Pages [layers, pages, kv_heads, page_size, head_dim], or of one layer without the first dimension."""
-    _check_half(what, k_pages=k_pages, v_pages=v_pages)
+    index = _check_half(what, "k_pages v_pages", k_pages, v_pages)
     if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
         raise ValueError(f"{what}: k_pages and v_pages must share one shape [layers, pages, kv_heads, page_size, "
                          f"head_dim], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     k = k_pages if k_pages.dim() == 5 else k_pages[None]
     v = v_pages if v_pages.dim() == 5 else v_pages[None]
-    if k.device != refs.device or k.shape[1] != refs.shape[0]:
-        raise ValueError(f"{what}: refs must have one entry per page ({k.shape[1]}) on {k.device}")
-    return (k.data_ptr(), _strides_of(k, range(4)), v.data_ptr(), _strides_of(v, range(4)), k.shape[0], k.shape[2],
-            k.shape[4])
+    layers, pages, hkv, _, hd = k.shape
+    if index != refs.get_device() or pages != refs.shape[0]:
+        raise ValueError(f"{what}: refs must have one entry per page ({pages}) on {k.device}")
+    return k.data_ptr(), _strides_of(k, 4), v.data_ptr(), _strides_of(v, 4), layers, hkv, hd
 
 
-def _cache_workspace(device, rows: int, pages: int, n: int = 0) -> torch.Tensor:
-    size = _lib.load().tk_cache_workspace(rows, pages, n)
+def _bytes(fn: str, *args) -> int:
+    """What a workspace function of the library answers, or its refusal raised."""
+    size = getattr(_lib.load(), fn)(*args)
     if size < 0:
-        raise _lib.TkError("tk_cache_workspace", size, _lib.load().tk_last_error_string().decode())
-    return torch.empty(size, dtype=torch.uint8, device=device)
+        raise _lib.TkError(fn, size, _lib.load().tk_last_error_string().decode())
+    return size
+
+
+def _plan_buffers(device, rows: int, pages: int, n: int = 0) -> tuple:
+    """The one-entry result of a bookkeeping call, and its workspace."""
+    size = _bytes("tk_cache_workspace", rows, pages, n)
+    return torch.empty(1, dtype=torch.int32, device=device), torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=None, key_valid=None):
@@ -538,29 +567,30 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=Non
     A sequence's bits do not depend on the batch.
     """
     what = "window_attention"
-    code = _check_half(what, q=q, k=k, v=v)
+    index = _check_half(what, "q k v", q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"{what}: q [B, H, Sq, hd] and k, v [B, Hkv, Sk, hd] expected, got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     b, h, sq, hd = q.shape
-    hkv, sk = k.shape[1], k.shape[2]
+    _, hkv, sk, _ = k.shape
     if out is None:
         out = torch.empty((b, sq, h * hd), dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (b, sq, h * hd):
-        raise ValueError(f"{what}: out must be [B, Sq, H*hd] = {(b, sq, h * hd)}, got {tuple(out.shape)}")
-    _check_half(what, q=q, out=out)
+    else:
+        _check_half(what, "q out", q, out)
+        if tuple(out.shape) != (b, sq, h * hd):
+            raise ValueError(f"{what}: out must be [B, Sq, H*hd] = {(b, sq, h * hd)}, got {tuple(out.shape)}")
     kv = None
     if key_valid is not None:
         if tuple(key_valid.shape) != (b, sk):
             raise ValueError(f"{what}: key_valid must be [B, Sk] = {(b, sk)}, got {tuple(key_valid.shape)}")
         kv = _row_mask(key_valid, b * sk)
-        if kv.device != q.device:
+        if kv.get_device() != index:
             raise ValueError(f"{what}: key_valid is on {kv.device}, not {q.device}")
-    o_strides = _lib.strides([out.stride(0) if b > 1 else 0, hd if h > 1 else 0, out.stride(1) if sq > 1 else 0])
+    o_strides = _strides_array((b, h, sq), (out.stride(0), hd, out.stride(1)), 3)
     _launch_on(
-        q.device, "window_attn", "tk_window_attn", q.data_ptr(), _strides_of(q, range(3)), k.data_ptr(),
-        _strides_of(k, range(3)), v.data_ptr(), _strides_of(v, range(3)), out.data_ptr(), o_strides, code, b, h, hkv,
-        sq, sk, hd, float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk,
+        index, "window_attn", "tk_window_attn", q.data_ptr(), _strides_of(q, 3), k.data_ptr(), _strides_of(k, 3),
+        v.data_ptr(), _strides_of(v, 3), out.data_ptr(), o_strides, _HALF_CODE[q.dtype], b, h, hkv, sq, sk, hd,
+        float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk,
     )
     return out
 
@@ -580,33 +610,31 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
     sequence's bits do not depend on the batch or ``max_length``.
     """
     what = "paged_attention"
-    code = _check_half(what, q=q, k_pages=k_pages, v_pages=v_pages)
+    index = _check_half(what, "q k_pages v_pages", q, k_pages, v_pages)
     if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or q.shape[2] != k_pages.shape[3]:
         raise ValueError(f"{what}: q [B, H, hd] and pages [pages, Hkv, page_size, hd] expected, got {tuple(q.shape)}, "
                          f"{tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
     b, h, hd = q.shape
     pages, hkv, page_size, _ = k_pages.shape
-    ptr, stride, width = _check_table(what, table, lengths)
-    if table.shape[0] != b or table.device != q.device:
-        raise ValueError(f"{what}: table must have a row per sequence ({b}) on {q.device}")
-    if max_length is None or batch_invariant:
-        max_length = width * page_size
+    ptr, stride, width, rows = _check_table(what, table, index)
+    if rows != b:
+        raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
+    lens = _check_int32(what, "lengths", lengths, index, b)
     if out is None:
         out = torch.empty((b, h * hd), dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (b, h * hd):
-        raise ValueError(f"{what}: out must be [B, H*hd] = {(b, h * hd)}, got {tuple(out.shape)}")
-    _check_half(what, q=q, out=out)
-    invariant = int(bool(batch_invariant))
-    size = _lib.load().tk_paged_attn_workspace(b, h, hkv, hd, int(max_length), int(window), int(sinks), invariant)
-    if size < 0:
-        raise _lib.TkError("tk_paged_attn_workspace", size, _lib.load().tk_last_error_string().decode())
+    else:
+        _check_half(what, "q out", q, out)
+        if tuple(out.shape) != (b, h * hd):
+            raise ValueError(f"{what}: out must be [B, H*hd] = {(b, h * hd)}, got {tuple(out.shape)}")
+    most = width * page_size if max_length is None or batch_invariant else int(max_length)
+    plan = (int(window), int(sinks), int(bool(batch_invariant)))
+    size = _bytes("tk_paged_attn_workspace", b, h, hkv, hd, most, *plan)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    o_strides = _lib.strides([out.stride(0) if b > 1 else 0, hd])
     _launch_on(
-        q.device, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_of(q, range(2)), k_pages.data_ptr(),
-        _strides_of(k_pages, range(3)), v_pages.data_ptr(), _strides_of(v_pages, range(3)), out.data_ptr(), o_strides,
-        code, b, h, hkv, hd, pages, page_size, ptr, stride, width, lengths.data_ptr(), int(max_length), float(scale),
-        int(window), int(sinks), invariant, ws.data_ptr() if ws is not None else None, size,
+        index, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_of(q, 2), k_pages.data_ptr(),
+        _strides_of(k_pages, 3), v_pages.data_ptr(), _strides_of(v_pages, 3), out.data_ptr(),
+        _strides_array((b, h), (out.stride(0), hd), 2), _HALF_CODE[q.dtype], b, h, hkv, hd, pages, page_size, ptr,
+        stride, width, lens, most, float(scale), *plan, ws.data_ptr() if size else None, size,
     )
     return out
 
@@ -622,23 +650,21 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
     ``lengths[b] - new[b] + i``.  Positions that have no page are left out.
     """
     what = "cache_append"
-    _check_half(what, k=k, v=v, k_pages=k_pages, v_pages=v_pages)
+    index = _check_half(what, "k v k_pages v_pages", k, v, k_pages, v_pages)
     if k.dim() != 4 or k.shape != v.shape or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
-            k.shape[2:] != (k_pages.shape[1], k_pages.shape[3]):
+            k.shape[2] != k_pages.shape[1] or k.shape[3] != k_pages.shape[3]:
         raise ValueError(f"{what}: k, v [B, n, Hkv, hd] and pages [pages, Hkv, page_size, hd] expected, got "
                          f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
     b, n, hkv, hd = k.shape
     pages, _, page_size, _ = k_pages.shape
-    ptr, stride, width = _check_table(what, table, lengths)
-    if table.shape[0] != b or table.device != k.device:
-        raise ValueError(f"{what}: table must have a row per sequence ({b}) on {k.device}")
-    if new is not None:
-        _check_int32(what, k.device, b, new=new)
+    ptr, stride, width, rows = _check_table(what, table, index)
+    if rows != b:
+        raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
     _launch_on(
-        k.device, "cache_append", "tk_cache_append", k.data_ptr(), _strides_of(k, range(3)), v.data_ptr(),
-        _strides_of(v, range(3)), k_pages.data_ptr(), _strides_of(k_pages, range(3)), v_pages.data_ptr(),
-        _strides_of(v_pages, range(3)), b, n, hkv, hd, pages, page_size, ptr, stride, width, lengths.data_ptr(),
-        new.data_ptr() if new is not None else None,
+        index, "cache_append", "tk_cache_append", k.data_ptr(), _strides_of(k, 3), v.data_ptr(), _strides_of(v, 3),
+        k_pages.data_ptr(), _strides_of(k_pages, 3), v_pages.data_ptr(), _strides_of(v_pages, 3), b, n, hkv, hd, pages,
+        page_size, ptr, stride, width, _check_int32(what, "lengths", lengths, index, b),
+        None if new is None else _check_int32(what, "new", new, index, b),
     )
 
 
@@ -654,11 +680,11 @@ def cache_reserve(table, lengths, refs, new, page_size: int):
     """
     what = "cache_reserve"
     state = _state_args(what, table, lengths, refs, page_size)
-    _check_int32(what, table.device, table.shape[0], new=new)
-    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0])
-    status = torch.empty(1, dtype=torch.int32, device=table.device)
-    _launch_on(table.device, "cache_reserve", "tk_cache_reserve", *state, new.data_ptr(), status.data_ptr(),
-               ws.data_ptr(), ws.numel())
+    index, rows = table.get_device(), state[3]
+    added = _check_int32(what, "new", new, index, rows)
+    status, ws, size = _plan_buffers(table.device, rows, refs.shape[0])
+    _launch_on(index, "cache_reserve", "tk_cache_reserve", *state, added, status.data_ptr(),
+               ws.data_ptr(), size)
     return status
 
 
@@ -676,13 +702,13 @@ def cache_fork(k_pages, v_pages, table, lengths, refs, parents, children):
     what = "cache_fork"
     cache = _cache_args(what, k_pages, v_pages, refs)
     state = _state_args(what, table, lengths, refs, k_pages.shape[-2])
-    _check_int32(what, table.device, parents=parents)
-    _check_int32(what, table.device, parents.shape[0], children=children)
+    index = table.get_device()
+    first = _check_int32(what, "parents", parents, index)
     n = parents.shape[0]
-    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0], n)
-    status = torch.empty(1, dtype=torch.int32, device=table.device)
-    _launch_on(table.device, "cache_fork", "tk_cache_fork", *cache, *state, parents.data_ptr(), children.data_ptr(), n,
-               status.data_ptr(), ws.data_ptr(), ws.numel())
+    second = _check_int32(what, "children", children, index, n)
+    status, ws, size = _plan_buffers(table.device, state[3], refs.shape[0], n)
+    _launch_on(index, "cache_fork", "tk_cache_fork", *cache, *state, first, second, n, status.data_ptr(),
+               ws.data_ptr(), size)
     return status
 
 
@@ -693,8 +719,8 @@ def cache_free(table, lengths, refs, rows, page_size: int) -> None:
     """
     what = "cache_free"
     state = _state_args(what, table, lengths, refs, page_size)
-    _check_int32(what, table.device, rows=rows)
-    _launch_on(table.device, "cache_free", "tk_cache_free", *state, rows.data_ptr(), rows.shape[0])
+    index = table.get_device()
+    _launch_on(index, "cache_free", "tk_cache_free", *state, _check_int32(what, "rows", rows, index), rows.shape[0])
 
 
 def cache_compact(k_pages, v_pages, table, lengths, refs):
@@ -708,8 +734,7 @@ def cache_compact(k_pages, v_pages, table, lengths, refs):
     what = "cache_compact"
     cache = _cache_args(what, k_pages, v_pages, refs)
     state = _state_args(what, table, lengths, refs, k_pages.shape[-2])
-    ws = _cache_workspace(table.device, table.shape[0], refs.shape[0])
-    used = torch.empty(1, dtype=torch.int32, device=table.device)
-    _launch_on(table.device, "cache_compact", "tk_cache_compact", *cache, *state, used.data_ptr(), ws.data_ptr(),
-               ws.numel())
+    used, ws, size = _plan_buffers(table.device, state[3], refs.shape[0])
+    _launch_on(table.get_device(), "cache_compact", "tk_cache_compact", *cache, *state, used.data_ptr(),
+               ws.data_ptr(), size)
     return used
