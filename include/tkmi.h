@@ -455,7 +455,16 @@ int tk_forward(const tk_model *model, const void *x, void *out, int64_t batch, i
  * q [batch, heads, q_len, head_dim], k and v [batch, kv_heads, k_len, head_dim], out as q:
  * element strides {b, h, s} in *_strides[3].  scale > 0.  What K and V hold at keys that
  * are not valid has no effect; at valid ones it must be finite.
+ * Launches with few query rows split their keys over workgroups and waves; batch_invariant:
+ * not so, a sequence's bits do not depend on the rest of the batch.  workspace:
+ * tk_window_attn_workspace bytes, 16-byte aligned, this call's own until its launches have
+ * run (0 bytes: may be NULL).
  */
+int64_t tk_window_attn_workspace(int64_t batch, int64_t heads,
+                                 int64_t kv_heads, int64_t q_len,
+                                 int64_t k_len, int64_t head_dim,
+                                 int64_t window, int64_t sinks,
+                                 int batch_invariant);
 int tk_window_attn(const void *q, const int64_t *q_strides, const void *k,
                    const int64_t *k_strides, const void *v,
                    const int64_t *v_strides, void *out,
@@ -463,7 +472,8 @@ int tk_window_attn(const void *q, const int64_t *q_strides, const void *k,
                    int64_t heads, int64_t kv_heads, int64_t q_len,
                    int64_t k_len, int64_t head_dim, float scale,
                    int64_t window, int64_t sinks, const uint8_t *key_valid,
-                   int64_t key_valid_stride, void *stream);
+                   int64_t key_valid_stride, int batch_invariant,
+                   void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * The cache: k and v pages [layers][pages][kv_heads][page_size][head_dim] (any strides with

@@ -36,11 +36,14 @@ def _window_inputs(b, h, hkv, sq, sk, hd, dtype, seed=0):
 
 def _check_window(q, k, v, window, sinks, valid=None, scale=None):
     scale = 1.5 * q.shape[3] ** -0.5 if scale is None else scale
-    got = ops.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), scale, window, sinks=sinks,
-                               key_valid=None if valid is None else valid.to(DEV))
     want, tol = window_reference(q, k, v, scale, window, sinks, valid)
-    _inside(got, want, tol)
-    return got
+    both = []
+    for invariant in (False, True):  # keys dealt to waves and workgroups where rows are few, and not
+        both.append(ops.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), scale, window, sinks=sinks,
+                                         key_valid=None if valid is None else valid.to(DEV),
+                                         batch_invariant=invariant))
+        _inside(both[-1], want, tol)
+    return torch.stack(both)
 
 
 # lengths around tiles (32 rows, 64 keys) and workgroups (128 rows); windows of one key, around tiles, past the keys
@@ -145,9 +148,23 @@ def test_window_of_every_key_is_flash_attention():
 def test_window_bits_do_not_depend_on_the_batch():
     for sq, sk, hd in [(260, 400, 64), (1, 900, 128), (40, 2000, 80)]:
         q, k, v = (t.to(DEV) for t in _window_inputs(40, 2, 1, sq, sk, hd, BF16, seed=sq))
-        whole = ops.window_attention(q, k, v, 0.1, 300, sinks=4)
+        whole = ops.window_attention(q, k, v, 0.1, 300, sinks=4, batch_invariant=True)
         for n in (0, 17):
-            assert torch.equal(ops.window_attention(q[n:n + 1], k[n:n + 1], v[n:n + 1], 0.1, 300, sinks=4)[0], whole[n])
+            assert torch.equal(ops.window_attention(q[n:n + 1], k[n:n + 1], v[n:n + 1], 0.1, 300, sinks=4,
+                                                    batch_invariant=True)[0], whole[n])
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 200])
+def test_window_few_rows_and_many_keys(hd):
+    """Keys split over workgroups: ends inside tiles, sinks, masks that leave some splits and some rows nothing."""
+    for sq, sk, window, sinks in [(1, 9000, 9000, 0), (3, 5000, 4999, 70), (40, 7001, 6000, 1), (2, 4097, 2048, 500)]:
+        q, k, v = _window_inputs(1, 2, 1, sq, sk, hd, F16 if sq % 2 else BF16, seed=sq + hd)
+        _check_window(q, k, v, window, sinks)
+        valid = torch.zeros(1, sk, dtype=torch.bool)
+        valid[:, sk // 2:sk // 2 + 300] = True
+        valid[:, sk - 1] = sq > 2
+        bad = ~valid[:, None, :, None].expand_as(k)
+        _check_window(q, k.masked_fill(bad, float("nan")), v.masked_fill(bad, float("inf")), window, sinks, valid)
 
 
 # ------------------------------------------------------------------- paged --

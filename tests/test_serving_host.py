@@ -13,9 +13,9 @@ S4 = _lib.strides([64, 64, 64, 64])
 
 
 def _window(dtype=1, b=1, h=4, hkv=2, sq=8, sk=8, hd=64, scale=0.1, window=4, sinks=0, q=16, k=16, strides=S3, kv=None,
-            kvs=0):
+            kvs=0, invariant=0, ws=None, size=0):
     return _lib.load().tk_window_attn(q, S3, k, strides, 16, S3, 16, S3, dtype, b, h, hkv, sq, sk, hd, scale, window,
-                                      sinks, kv, kvs, None)
+                                      sinks, kv, kvs, invariant, ws, size, None)
 
 
 @pytest.mark.parametrize("call,code", [
@@ -23,6 +23,8 @@ def _window(dtype=1, b=1, h=4, hkv=2, sq=8, sk=8, hd=64, scale=0.1, window=4, si
     (dict(sinks=-1), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1),
     (dict(hd=12), -2), (dict(hd=264), -2), (dict(q=None), -1), (dict(k=24), -2), (dict(b=-1), -1),
     (dict(strides=_lib.strides([64, 64, 60])), -2), (dict(kv=16, kvs=7), -1), (dict(sk=1 << 30), -1),
+    (dict(sk=100000, window=100000), -1),  # splits its keys and has no workspace
+    (dict(sk=100000, window=100000, ws=8, size=1 << 30), -1), (dict(sk=100000, window=100000, ws=16, size=64), -1),
     (dict(b=0), 0), (dict(sq=0), 0), (dict(h=0, hkv=0), 0),
 ])
 def test_window_attention_refuses(call, code):
@@ -48,6 +50,17 @@ def _paged(dtype=1, b=2, h=4, hkv=2, hd=64, pages=8, ps=16, table=16, stride=4, 
 def test_paged_attention_refuses(call, code):
     assert _paged(**call) == code
     assert code == 0 or _lib.load().tk_last_error_string().decode()
+
+
+def test_window_workspace():
+    size = _lib.load().tk_window_attn_workspace
+    assert size(1, 4, 4, 5, 100000, 64, 100000, 0, 1) == 0  # batch-invariant: no split
+    assert size(64, 16, 4, 500, 500, 64, 100, 4, 0) == 0    # enough rows
+    assert size(1, 4, 4, 5, 100, 64, 20, 0, 0) == 0         # few keys: one workgroup's waves share them
+    assert size(1, 4, 4, 5, 100000, 64, 100000, 0, 0) % (4 * 5 * 66 * 4) == 0
+    assert size(1, 4, 4, 5, 100000, 64, 100000, 0, 0) > size(1, 4, 4, 5, 100000, 64, 4000, 0, 0) > 0
+    assert size(1, 4, 4, 5, 100000, 64, 1 << 60, 0, 0) == size(1, 4, 4, 5, 100000, 64, 100000, 0, 0)
+    assert size(0, 4, 4, 5, 10, 64, 4, 0, 0) == 0 and size(1, 4, 4, 5, 4, 64, 4, 0, 0) == -1
 
 
 def test_paged_workspace():

@@ -18,11 +18,6 @@
 namespace tk {
 namespace {
 
-// s_waitcnt lgkmcnt(0): this wave's LDS reads have returned.
-__device__ __forceinline__ void wait_lds_reads() {
-  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
-}
-
 template <int HD, int NW, bool CAUSAL, bool KMASK, typename Args>
 __device__ __forceinline__ void keysplit_body(const Args& p) {
   constexpr int BN = HD <= 128 ? 64 : 32;  // keys per tile

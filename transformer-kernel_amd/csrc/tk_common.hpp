@@ -68,6 +68,11 @@ __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
+// s_waitcnt lgkmcnt(0): this wave's LDS reads have returned and its writes are done.
+__device__ __forceinline__ void wait_lds_reads() {
+  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+}
+
 // Workgroup barrier without the memory fence of __syncthreads() (which
 // waits for every outstanding vector-memory op, i.e. drains all in-flight
 // tile copies).  The empty asm statements keep the compiler from moving LDS

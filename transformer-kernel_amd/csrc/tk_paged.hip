@@ -25,7 +25,7 @@
 // Numerics: fp32 scores, maxima, sums and O.  P is rounded to 16 bits for the product: fp16
 // (half a step 2^-11 of the weight) as it is; bf16 (2^-8) as the sum of two bf16 numbers, whose
 // second product the idle matrix cores do for nothing.
-#include "tk_elem.hpp"
+#include "tk_join.hpp"
 
 namespace tk {
 namespace {
@@ -305,59 +305,6 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedArgs p) {
   paged_body<T, DT, NW>(p);
 }
 
-// Joins a row's splits: one workgroup per (sequence, query head), kJoin / lpr groups of lpr lanes
-// of 4 columns, group i taking splits i, i + groups, ...; the groups are added in their order, so the
-// sums have one order whatever the batch.  (One wave that walked the splits alone took 235 us for
-// 391 of them.)
-constexpr int kJoin = 512;
-template <typename T>
-__global__ __launch_bounds__(kJoin) void paged_join_kernel(PagedArgs p) {
-  __shared__ float m_lds[kJoin / 64];
-  __shared__ f32x4 o_lds[kJoin];
-  __shared__ float l_lds[kJoin];
-  const int64_t rowid = blockIdx.x;
-  const int b = (int)(rowid / p.heads), h = (int)(rowid % p.heads);
-  const float* st = p.stats + 2 * rowid * p.splits;
-  float m = -INFINITY;
-  for (int s = threadIdx.x; s < p.splits; s += kJoin) m = fmaxf(m, st[2 * s]);
-  m = group_max<64>(m);
-  if ((threadIdx.x & 63) == 0) m_lds[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoin / 64; ++w) m = fmaxf(m, m_lds[w]);
-  const float m_ref = m == -INFINITY ? 0.f : m;
-
-  const int lpr = p.hd <= 64 ? 16 : p.hd <= 128 ? 32 : 64, groups = kJoin / lpr;
-  const int grp = threadIdx.x / lpr, d = (threadIdx.x % lpr) * 4;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  if (d < p.hd) {
-    const float* part = p.part + rowid * p.splits * p.hd + d;
-#pragma unroll 4
-    for (int s = grp; s < p.splits; s += groups) {
-      const float f = __builtin_amdgcn_exp2f(st[2 * s] - m_ref);
-      if (st[2 * s] == -INFINITY) continue;  // an empty split wrote no O
-      const f32x4 o = *reinterpret_cast<const f32x4*>(part + (int64_t)s * p.hd);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, o[e], sum[e]);
-      l = fmaf(f, st[2 * s + 1], l);
-    }
-  }
-  o_lds[threadIdx.x] = sum;
-  l_lds[threadIdx.x] = l;
-  __syncthreads();
-  if (grp != 0 || d >= p.hd) return;
-  for (int i = 1; i < groups; ++i) {
-    const f32x4 o = o_lds[i * lpr + threadIdx.x];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += o[e];
-    l += l_lds[i * lpr + threadIdx.x];
-  }
-  T* out = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : sum[e] / l);
-}
-
 constexpr int kPagedWaves = 4;
 
 // Tiles of 32 keys a workgroup takes, and the splits that this makes of a sequence of max_length keys.
@@ -390,9 +337,17 @@ int launch_paged(const PagedArgs& p, int64_t grid, hipStream_t st) {
   else hipLaunchKernelGGL((paged_attn_kernel<T, 256, NW>), g, blk, 0, st, p);
   int rc = check_launch("tk_paged_attn");
   if (rc != TK_OK || p.splits == 1) return rc;
-  hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)((int64_t)p.batch * p.heads)), dim3(kJoin), 0,
-                     st, p);
-  return check_launch("tk_paged_attn");
+  JoinArgs j{};
+  j.part = p.part;
+  j.stats = p.stats;
+  j.o = p.o;
+  j.os[0] = p.os[0];
+  j.os[1] = p.os[1];
+  j.heads = p.heads;
+  j.q_len = 1;
+  j.hd = p.hd;
+  j.splits = p.splits;
+  return launch_join<T>("tk_paged_attn", j, (int64_t)p.batch * p.heads, st);
 }
 
 }  // namespace

@@ -19,7 +19,7 @@
 // step: fp16 2^-11, bf16 2^-8 of the weight), the sum taken of the rounded weights, so that they
 // add up to 1.
 #include "tk_attn_tile.hpp"
-#include "tk_elem.hpp"
+#include "tk_join.hpp"
 
 namespace tk {
 namespace {
@@ -34,7 +34,23 @@ struct WindowArgs {
   int64_t qs[3], ks[3], vs[3], os[3];  // elements, {b, h, s}
   int batch, heads, group, q_len, k_len, hd, window, sinks;
   int n_qt;
+  int splits, per_split;  // window_split_kernel: key tiles of a workgroup
+  float* part;            // its results where splits > 1 (tk_join.hpp)
+  float* stats;
   float scale_log2;
+};
+
+// The key tiles that rows at positions [first, last] see: those of the sinks, then those of the windows.
+template <int BN>
+struct TileList {
+  int st, wt, n;
+  __device__ __forceinline__ TileList(const WindowArgs& p, int first, int last) {
+    const int lo = max(0, first - p.window + 1);
+    wt = lo / BN;
+    st = min((min(p.sinks, lo) + BN - 1) / BN, wt);
+    n = st + last / BN + 1 - wt;
+  }
+  __device__ __forceinline__ int key(int t) const { return (t < st ? t : t - st + wt) * BN; }
 };
 
 template <typename T, int DT, int BN, int NW, bool KMASK>
@@ -68,12 +84,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
   const int row = q0 + wave * 32 + (lane & 31);
   const int pos = shift + row;
   const int w_lo = shift + q0 + wave * 32, w_hi = w_lo + 31;                    // positions of the wave's rows
-  const int g_hi = min(shift + q0 + 32 * NW - 1, p.k_len - 1);                  // last position of the workgroup's
-  const int lo = max(0, shift + q0 - p.window + 1);                             // first key of any of its windows
-  const int wt = lo / BN;
-  const int st = min((min(p.sinks, lo) + BN - 1) / BN, wt);
-  const int n_kt = st + (g_hi / BN + 1) - wt;
-  auto tile_key = [&](int t) { return (t < st ? t : t - st + wt) * BN; };
+  const TileList<BN> tiles(p, shift + q0, min(shift + q0 + 32 * NW - 1, p.k_len - 1));
 
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + kvh * p.ks[1];
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + kvh * p.vs[1];
@@ -94,7 +105,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
     vp[i] = vb + r * p.vs[2] + min(phys ^ vswz<RB>(r), last_chunk) * 8;
   }
   auto copy = [&](int t, uint32_t dst) {
-    const int k0 = tile_key(t);
+    const int k0 = tiles.key(t);
     const int64_t ko = k0 * p.ks[2], vo = k0 * p.vs[2];
     if (k0 + BN <= p.k_len) {
 #pragma unroll
@@ -141,8 +152,8 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
   const float cs = p.scale_log2;
 
   copy(0, lds0);
-  for (int t = 0; t < n_kt; ++t) {
-    const int k0 = tile_key(t);
+  for (int t = 0; t < tiles.n; ++t) {
+    const int k0 = tiles.key(t);
     char* ks_ = smem + (t & 1) * 2 * TILE;
     char* vs_ = ks_ + TILE;
     uint64_t bits = ~0ull;
@@ -151,17 +162,17 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
       bits = __ballot(lane < BN && key < p.k_len && kvb[min(key, p.k_len - 1)] != 0);
     }
     wait_vmcnt<0>();
-    if (KMASK && bits != (BN == 64 ? ~0ull : (1ull << BN) - 1)) {
+    if (KMASK && bits != ~0ull >> (64 - BN)) {
       // whatever lies in rows that are not valid times a weight of 0 must be 0
 #pragma unroll
       for (int i = 0; i < COPIES; ++i) {
         const int c = wave * COPIES + i;
         if (!((bits >> (c * RPC + lane / CPR)) & 1)) *reinterpret_cast<u32x4*>(vs_ + c * 1024 + lane * 16) = u32x4{};
       }
-      __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+      wait_lds_reads();
     }
     lds_barrier();
-    if (t + 1 < n_kt) copy(t + 1, lds0 + ((t + 1) & 1) * 2 * TILE);
+    if (t + 1 < tiles.n) copy(t + 1, lds0 + ((t + 1) & 1) * 2 * TILE);
     // nothing of this tile for any of the wave's rows
     if (k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
 
@@ -232,29 +243,293 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
   }
 }
 
+// The same rows' keys dealt to the waves of a workgroup (and to several workgroups): for launches with too
+// few query rows to fill the chip, whose workgroups of the kernel above would walk their tiles as one
+// serial chain each.  32 rows of one head per workgroup; wave w takes every NW-th of its tiles, into K and V
+// slots of its own, so the loop has no barrier: the next K is copied when the current one's products
+// are done, the next V after P.V.  At the end the waves' (max, sum, O) are merged in wave order.
+template <typename T, int DT, int BN, int NW, bool KMASK>
+__device__ __forceinline__ void window_split_body(const WindowArgs& p) {
+  typedef typename Elem<T>::x8 x8;
+  typedef typename Elem<T>::x4 x4;
+  constexpr int NB = BN / 32;
+  constexpr int RB = DT * 2;
+  constexpr int CPR = RB / 16;
+  constexpr int TILE = BN * RB;
+  constexpr int COPIES = TILE / 1024;
+  constexpr int RPC = 1024 / RB;
+  constexpr int DB = DT / 32;
+  constexpr int KSTEPS = DT / 16;
+  constexpr int SLOT = 2 * TILE;
+  constexpr int CHUNKS = 4 * DB;  // 4-register pieces of O
+  static_assert(CHUNKS * 1024 <= SLOT && CHUNKS % NW == 0, "a wave's O fits its slots, whole pieces per wave");
+  __shared__ __attribute__((aligned(16))) char smem[NW * SLOT];
+  __shared__ float row_m[NW][32], row_l[NW][32];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 5;
+  int id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int qt = id % p.n_qt, bh = id / p.n_qt;
+  const int b = bh / p.heads, h = bh % p.heads, kvh = h / p.group;
+
+  const int q0 = qt * 32, shift = p.k_len - p.q_len;
+  const int row = q0 + (lane & 31), pos = shift + row;
+  const int w_lo = shift + q0, w_hi = min(w_lo + 31, p.k_len - 1);
+  const TileList<BN> tiles(p, w_lo, w_hi);
+  const int t_end = min(tiles.n, (split + 1) * p.per_split);
+  int t = split * p.per_split + wave;
+
+  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + kvh * p.ks[1];
+  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + kvh * p.vs[1];
+  const uint8_t* kvb = KMASK ? p.kv + b * p.kvs : nullptr;
+  char* ks_ = smem + wave * SLOT;
+  char* vs_ = ks_ + TILE;
+  const uint32_t k_lds = (uint32_t)(size_t)(lds_char*)ks_, v_lds = k_lds + TILE;
+  const int last_chunk = p.hd / 8 - 1;
+
+  auto copy = [&](const T* base, int64_t rs, int k0, uint32_t dst, bool is_v) {  // as in window_body
+    const T* tile = base + k0 * rs;
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      const int r = c * RPC + lane / CPR, phys = lane % CPR;
+      const int chunk = is_v ? phys ^ vswz<RB>(r) : (swz_off<RB>(r, phys) - r * RB) >> 4;
+      dma16(tile + min(r, p.k_len - 1 - k0) * rs + min(chunk, last_chunk) * 8, dst + c * 1024);
+    }
+  };
+
+  x8 qf[KSTEPS];
+  {
+    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + (int64_t)min(row, p.q_len - 1) * p.qs[2];
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      const int d = 16 * kk + 8 * g;
+      qf[kk] = x8{};
+      if (d < p.hd) qf[kk] = *reinterpret_cast<const x8*>(qr + d);
+    }
+  }
+  if (t < t_end) {
+    copy(kb, p.ks[2], tiles.key(t), k_lds, false);
+    copy(vb, p.vs[2], tiles.key(t), v_lds, true);
+  }
+  int v_rd[2][DB];  // transposed V reads, as attend_one_tile
+  {
+    const int tq = lane >> 4, ts = lane & 15;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int vr = 8 * r + 4 * (tq >> 1) + (ts >> 2);
+        const int col = 32 * d + 16 * (tq & 1) + 4 * (ts & 3);
+        v_rd[r][d] = vr * RB + (((col >> 3) ^ vswz<RB>(vr)) << 4) + (col & 7) * 2;
+      }
+  }
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float cs = p.scale_log2;
+
+  for (; t < t_end; t += NW) {
+    const int k0 = tiles.key(t);
+    const bool more = t + NW < t_end;
+    int byte = 1;
+    if (KMASK) byte = lane < BN && k0 + lane < p.k_len ? kvb[k0 + lane] : 0;
+    wait_vmcnt<COPIES>();  // all but V's copies (or fewer, if the validity byte went out before): K has landed
+    asm volatile("" ::: "memory");
+    f32x16 s[NB];
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+      for (int kb2 = 0; kb2 < NB; ++kb2) {
+        const x8 kf = *reinterpret_cast<const x8*>(ks_ + swz_off<RB>(kb2 * 32 + (lane & 31), 2 * kk + g));
+        s[kb2] = Elem<T>::mfma32(kf, qf[kk], kk == 0 ? f32x16{} : s[kb2]);
+      }
+    // every K fragment is in registers: the slot may be refilled
+    asm volatile("" ::: "memory");
+    wait_lds_reads();
+    const uint64_t bits = KMASK ? (uint64_t)__ballot(byte != 0) : ~0ull;  // waits for the byte, and so for V
+    if (more) copy(kb, p.ks[2], tiles.key(t + NW), k_lds, false);
+
+    const bool whole = k0 + BN - 1 <= w_lo && (k0 > w_lo + 31 - p.window || k0 + BN <= p.sinks);
+    if (KMASK || !whole) {
+      const uint64_t kbits = bits >> (4 * g);
+#pragma unroll
+      for (int e = 0; e < 16 * NB; ++e) {
+        const int j = (e >> 4) * 32 + 8 * ((e & 15) >> 2) + (e & 3), key = k0 + j + 4 * g;
+        const bool see = key <= pos && (key > pos - p.window || key < p.sinks) && (!KMASK || ((kbits >> j) & 1));
+        if (!see) s[e >> 4][e & 15] = -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16 * NB; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+    const float m_tile = pair_max(mx) * cs;
+    if (__ballot(m_tile > m_run + 8.f) != 0ull) {
+      const float m_new = fmaxf(m_run, m_tile);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf[2 * NB];
+#pragma unroll
+    for (int e = 0; e < 16 * NB; ++e)
+      pf[e >> 3][e & 7] = (T)__builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], cs, -m_use));
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) l_run = Elem<T>::sum8(pf[i], l_run);
+
+    if (more) wait_vmcnt<COPIES>();  // all but the next K's copies
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    if (KMASK && bits != ~0ull >> (64 - BN)) {
+      // whatever lies in rows that are not valid times a weight of 0 must be 0
+#pragma unroll
+      for (int c = 0; c < COPIES; ++c)
+        if (!((bits >> (c * RPC + lane / CPR)) & 1)) *reinterpret_cast<u32x4*>(vs_ + c * 1024 + lane * 16) = u32x4{};
+      wait_lds_reads();
+      asm volatile("" ::: "memory");
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * NB * DB; ++c) {
+      const int t16 = c / DB, d = c % DB;
+      const lds_char* base = (const lds_char*)(vs_ + t16 * 16 * RB);
+      const tr_f16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_f16x4*)(base + v_rd[0][d]));
+      const tr_f16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_f16x4*)(base + v_rd[1][d]));
+      const f16x8 vf = __builtin_shufflevector(__builtin_bit_cast(f16x4, lo4), __builtin_bit_cast(f16x4, hi4), 0, 1, 2,
+                                               3, 4, 5, 6, 7);
+      acc[d] = Elem<T>::mfma32(__builtin_bit_cast(x8, vf), pf[t16], acc[d]);
+    }
+    asm volatile("" ::: "memory");
+    wait_lds_reads();
+    if (more) copy(vb, p.vs[2], tiles.key(t + NW), v_lds, true);
+  }
+
+  // ---- merge: a wave writes its O (CHUNKS of 64 lanes x 16 bytes) into its own slots ----
+  asm volatile("" ::: "memory");
+  l_run = pair_sum(l_run);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const f32x16& o = acc[c / 4];
+    const int q = c % 4;
+    *reinterpret_cast<f32x4*>(ks_ + c * 1024 + lane * 16) = f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
+  }
+  if (g == 0) {
+    row_m[wave][lane] = m_run;
+    row_l[wave][lane] = l_run;
+  }
+  __syncthreads();
+  float f[NW], m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    f[w] = row_m[w][lane & 31];
+    m_all = fmaxf(m_all, f[w]);
+  }
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(f[w] - m_ref);
+    l_all = fmaf(f[w], row_l[w][lane & 31], l_all);
+  }
+  if (row >= p.q_len) return;
+  const float inv = l_all == 0.f ? 0.f : 1.0f / l_all;
+  T* orow = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
+  const int64_t part = ((int64_t)bh * p.q_len + row) * p.splits + split;
+  if (p.splits > 1 && wave == 0 && g == 0) {
+    p.stats[2 * part] = m_all;
+    p.stats[2 * part + 1] = l_all;
+  }
+#pragma unroll
+  for (int c0 = 0; c0 < CHUNKS; c0 += NW) {
+    const int c = c0 + wave, dd = (c / 4) * 32 + 8 * (c % 4) + 4 * g;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(smem + w * SLOT + c * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f[w], v[e], o[e]);
+    }
+    if (dd >= p.hd) continue;
+    if (p.splits > 1) *reinterpret_cast<f32x4*>(p.part + part * p.hd + dd) = o;
+    else *reinterpret_cast<x4*>(orow + dd) = x4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+  }
+}
+
+template <typename T, int DT, int BN, int NW, bool KMASK>
+__global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_split_kernel(WindowArgs p) {
+  window_split_body<T, DT, BN, NW, KMASK>(p);
+}
+
 template <typename T, int DT, int BN, int NW, bool KMASK>
 __global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_attn_kernel(WindowArgs p) {
   window_body<T, DT, BN, NW, KMASK>(p);
 }
 
-template <typename T, int DT, int BN>
-int launch_window(WindowArgs p, hipStream_t st) {
+constexpr int kSplitWaves = 4;
+
+// Which kernel, and over how many workgroups window_split_kernel deals a block of 32 rows' keys.
+struct WindowPlan {
+  bool split;
+  int64_t splits, per_split;
+};
+WindowPlan window_plan(int64_t bh, int64_t q_len, int64_t k_len, int64_t window, int64_t sinks, int64_t hd,
+                       bool batch_invariant) {
+  if (batch_invariant || bh * ((q_len + 127) / 128) > 256) return {false, 1, 0};
+  const int64_t bn = hd <= 64 ? 64 : 32;
+  int64_t keys = window + 31 + sinks;
+  if (keys > k_len) keys = k_len;
+  const int64_t tiles = (keys + bn - 1) / bn + 2;  // the sinks and the windows may begin and end inside tiles
+  const int64_t want = (512 + bh * ((q_len + 31) / 32) - 1) / (bh * ((q_len + 31) / 32));
+  int64_t per = (tiles + want - 1) / want;
+  per = (per + kSplitWaves - 1) / kSplitWaves * kSplitWaves;
+  if (per < 2 * kSplitWaves) per = 2 * kSplitWaves;
+  return {true, (tiles + per - 1) / per, per};
+}
+
+template <typename T, int DT, int BN, int BNS>
+int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   constexpr int NW = 4;
-  p.n_qt = (p.q_len + 32 * NW - 1) / (32 * NW);
-  const int64_t total = (int64_t)p.n_qt * p.batch * p.heads;
-  TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "tk_window_attn: too many workgroups");
-  const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
-  if (p.kv) hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, true>), g, blk, 0, st, p);
-  else hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, false>), g, blk, 0, st, p);
-  return check_launch("tk_window_attn");
+  const char* fn = "tk_window_attn";
+  const int rows = plan.split ? 32 : 32 * NW;
+  p.n_qt = (p.q_len + rows - 1) / rows;
+  const int64_t total = (int64_t)p.n_qt * p.batch * p.heads * plan.splits;
+  TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  if (!plan.split) {
+    const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
+    if (p.kv) hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, true>), g, blk, 0, st, p);
+    else hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, false>), g, blk, 0, st, p);
+    return check_launch(fn);
+  }
+  const dim3 g((unsigned)total), blk(kSplitWaves * 64);
+  if (p.kv) hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kSplitWaves, true>), g, blk, 0, st, p);
+  else hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kSplitWaves, false>), g, blk, 0, st, p);
+  const int rc = check_launch(fn);
+  if (rc != TK_OK || p.splits == 1) return rc;
+  JoinArgs j{};
+  j.part = p.part;
+  j.stats = p.stats;
+  j.o = p.o;
+  for (int i = 0; i < 3; ++i) j.os[i] = p.os[i];
+  j.heads = p.heads;
+  j.q_len = p.q_len;
+  j.hd = p.hd;
+  j.splits = p.splits;
+  return launch_join<T>(fn, j, (int64_t)p.batch * p.heads * p.q_len, st);
 }
 
 template <typename T>
-int dispatch_window(const WindowArgs& p, hipStream_t st) {
-  if (p.hd <= 32) return launch_window<T, 32, 64>(p, st);
-  if (p.hd <= 64) return launch_window<T, 64, 64>(p, st);
-  if (p.hd <= 128) return launch_window<T, 128, 64>(p, st);
-  return launch_window<T, 256, 32>(p, st);
+int dispatch_window(const WindowArgs& p, const WindowPlan& plan, hipStream_t st) {
+  if (p.hd <= 32) return launch_window<T, 32, 64, 64>(p, plan, st);
+  if (p.hd <= 64) return launch_window<T, 64, 64, 64>(p, plan, st);
+  if (p.hd <= 128) return launch_window<T, 128, 64, 32>(p, plan, st);
+  return launch_window<T, 256, 32, 32>(p, plan, st);
 }
 
 }  // namespace
@@ -262,39 +537,71 @@ int dispatch_window(const WindowArgs& p, hipStream_t st) {
 
 using namespace tk;
 
-extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                              const void* v, const int64_t* v_strides, void* out, const int64_t* o_strides, int dtype,
-                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t k_len,
-                              int64_t head_dim, float scale, int64_t window, int64_t sinks, const uint8_t* key_valid,
-                              int64_t key_valid_stride, void* stream) {
-  const char* fn = "tk_window_attn";
-  TK_REQUIRE(dtype == TK_F16 || dtype == TK_BF16, TK_ERR_ARG, "%s: dtype %d is not TK_F16 or TK_BF16", fn, dtype);
+namespace {
+
+int check_window_shape(const char* fn, int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t k_len,
+                       int64_t head_dim, int64_t window, int64_t sinks) {
   TK_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 0 && q_len >= 0 && head_dim >= 0 && sinks >= 0 &&
                  batch < (1ll << 31) && heads < (1ll << 31) && kv_heads < (1ll << 31),
              TK_ERR_ARG, "%s: size out of range", fn);
   TK_REQUIRE(q_len <= k_len && k_len < (1ll << 30), TK_ERR_ARG, "%s: q_len=%lld, k_len=%lld: at most k_len queries", fn,
              (long long)q_len, (long long)k_len);
   TK_REQUIRE(window >= 1, TK_ERR_ARG, "%s: window=%lld < 1", fn, (long long)window);
-  TK_REQUIRE(scale > 0.f && scale <= 3.0e38f, TK_ERR_ARG, "%s: scale must be positive and finite", fn);
   TK_REQUIRE(kv_heads == 0 ? heads == 0 : heads % kv_heads == 0, TK_ERR_ARG,
              "%s: heads=%lld is no multiple of kv_heads=%lld", fn, (long long)heads, (long long)kv_heads);
   TK_REQUIRE(head_dim <= 256 && head_dim % 8 == 0, TK_ERR_UNSUPPORTED,
              "%s: head_dim=%lld is no multiple of 8 up to 256", fn, (long long)head_dim);
+  TK_REQUIRE(batch * heads < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many heads in all", fn);
+  return TK_OK;
+}
+
+// Past every key a window changes nothing, nor do sinks; kept small enough for sums of positions.
+int64_t at_most(int64_t x, int64_t k_len) { return x < k_len ? x : k_len; }
+
+int64_t window_workspace(const WindowPlan& plan, int64_t rows, int64_t head_dim) {
+  return plan.splits == 1 ? 0 : rows * plan.splits * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+}  // namespace
+
+extern "C" int64_t tk_window_attn_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len,
+                                            int64_t k_len, int64_t head_dim, int64_t window, int64_t sinks,
+                                            int batch_invariant) {
+  const int rc = check_window_shape("tk_window_attn_workspace", batch, heads, kv_heads, q_len, k_len, head_dim, window,
+                                    sinks);
+  if (rc != TK_OK) return rc;
+  if (batch == 0 || heads == 0 || q_len == 0) return 0;
+  return window_workspace(window_plan(batch * heads, q_len, k_len, at_most(window, k_len), at_most(sinks, k_len),
+                                      head_dim, batch_invariant != 0),
+                          batch * heads * q_len, head_dim);
+}
+
+extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                              const void* v, const int64_t* v_strides, void* out, const int64_t* o_strides, int dtype,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t k_len,
+                              int64_t head_dim, float scale, int64_t window, int64_t sinks, const uint8_t* key_valid,
+                              int64_t key_valid_stride, int batch_invariant, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  const char* fn = "tk_window_attn";
+  TK_REQUIRE(dtype == TK_F16 || dtype == TK_BF16, TK_ERR_ARG, "%s: dtype %d is not TK_F16 or TK_BF16", fn, dtype);
+  const int rc = check_window_shape(fn, batch, heads, kv_heads, q_len, k_len, head_dim, window, sinks);
+  if (rc != TK_OK) return rc;
+  TK_REQUIRE(scale > 0.f && scale <= 3.0e38f, TK_ERR_ARG, "%s: scale must be positive and finite", fn);
   if (batch == 0 || heads == 0 || q_len == 0 || head_dim == 0) return TK_OK;
   TK_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides && o_strides, TK_ERR_ARG, "%s: null pointer", fn);
   TK_REQUIRE(key_valid == nullptr || key_valid_stride >= k_len, TK_ERR_ARG, "%s: key_valid_stride=%lld < k_len", fn,
              (long long)key_valid_stride);
   auto al = [](const void* ptr, uintptr_t a) { return ((uintptr_t)ptr % a) == 0; };
-  bool rows = al(q, 16) && al(k, 16) && al(v, 16) && al(out, 8);
+  bool vecs = al(q, 16) && al(k, 16) && al(v, 16) && al(out, 8);
   WindowArgs p{};
   for (int i = 0; i < 3; ++i) {
-    rows = rows && q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
+    vecs = vecs && q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
     p.qs[i] = q_strides[i];
     p.ks[i] = k_strides[i];
     p.vs[i] = v_strides[i];
     p.os[i] = o_strides[i];
   }
-  TK_REQUIRE(rows, TK_ERR_UNSUPPORTED, "%s: rows of q, k, v must be 16-byte aligned, of out 8-byte", fn);
+  TK_REQUIRE(vecs, TK_ERR_UNSUPPORTED, "%s: rows of q, k, v must be 16-byte aligned, of out 8-byte", fn);
   p.q = q;
   p.k = k;
   p.v = v;
@@ -307,9 +614,17 @@ extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const voi
   p.q_len = (int)q_len;
   p.k_len = (int)k_len;
   p.hd = (int)head_dim;
-  // past every key both change nothing; kept small enough for sums of positions
-  p.window = (int)(window < k_len ? window : k_len);
-  p.sinks = (int)(sinks < k_len ? sinks : k_len);
+  p.window = (int)at_most(window, k_len);
+  p.sinks = (int)at_most(sinks, k_len);
   p.scale_log2 = scale * 1.4426950408889634f;
-  return dtype == TK_F16 ? dispatch_window<f16>(p, as_stream(stream)) : dispatch_window<bf16>(p, as_stream(stream));
+  const WindowPlan plan = window_plan(batch * heads, q_len, k_len, p.window, p.sinks, head_dim, batch_invariant != 0);
+  const int64_t rows = batch * heads * q_len, need = window_workspace(plan, rows, head_dim);
+  TK_REQUIRE(need == 0 || (workspace && al(workspace, 16) && workspace_bytes >= need), TK_ERR_ARG,
+             "%s: workspace of %lld bytes, 16-byte aligned, needed", fn, (long long)need);
+  p.splits = (int)plan.splits;
+  p.per_split = (int)plan.per_split;
+  p.part = reinterpret_cast<float*>(workspace);
+  p.stats = need ? p.part + rows * plan.splits * head_dim : nullptr;
+  return dtype == TK_F16 ? dispatch_window<f16>(p, plan, as_stream(stream))
+                         : dispatch_window<bf16>(p, plan, as_stream(stream));
 }

@@ -121,8 +121,10 @@ SIGNATURES = {
     ),
     "tk_window_attn": (
         c_int,
-        [c_void_p, _STRIDES] * 4 + [c_int] + [c_int64] * 6 + [c_float, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+        [c_void_p, _STRIDES] * 4 + [c_int] + [c_int64] * 6
+        + [c_float, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p],
     ),
+    "tk_window_attn_workspace": (c_int64, [c_int64] * 8 + [c_int]),
     "tk_paged_attn_workspace": (c_int64, [c_int64] * 7 + [c_int]),
     "tk_paged_attn": (
         c_int,

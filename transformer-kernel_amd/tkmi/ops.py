@@ -447,6 +447,7 @@ def masked_softmax(scores, causal: bool, key_len=None, heads_per_batch: int = 1)
 # --------------------------------------------------------------------------- #
 
 _HALF_CODE = {torch.float16: TK_F16, torch.bfloat16: TK_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 # A decode step is a few calls of some microseconds per layer, so what a call does on the host is
 # kept short: one pass over the tensors that are all right, and descriptions of what is wrong
@@ -455,7 +456,7 @@ _HALF_CODE = {torch.float16: TK_F16, torch.bfloat16: TK_BF16}
 
 def _launch_on(index: int, name: str, fn: str, *args) -> None:
     """A launch on the current stream of device ``index``, with that device current."""
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = _raw_stream(index)  # torch.cuda.current_stream(index).cuda_stream, without the object (1.1 us)
     if index == torch.cuda.current_device():
         _launch(name, fn, *args, stream)
     else:
@@ -547,13 +548,14 @@ def _bytes(fn: str, *args) -> int:
     return size
 
 
-def _plan_buffers(device, rows: int, pages: int, n: int = 0) -> tuple:
+def _plan_buffers(table, rows: int, pages: int, n: int = 0) -> tuple:
     """The one-entry result of a bookkeeping call, and its workspace."""
     size = _bytes("tk_cache_workspace", rows, pages, n)
-    return torch.empty(1, dtype=torch.int32, device=device), torch.empty(size, dtype=torch.uint8, device=device), size
+    return table.new_empty(1), table.new_empty(size // 4), size
 
 
-def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=None, key_valid=None):
+def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=None, key_valid=None,
+                     batch_invariant: bool = False):
     """Causal attention over the last ``window`` keys and the first ``sinks``; returns ``[B, Sq, H*hd]``.
 
     q is ``[B, H, Sq, hd]``, k and v ``[B, Hkv, Sk, hd]`` with ``Sq <= Sk`` and ``H`` a
@@ -564,7 +566,7 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=Non
     or ``j < sinks``.  ``key_valid`` (optional ``[B, Sk]`` bool): other keys are not seen,
     whatever they hold; at valid ones K and V must be finite.  A query that sees nothing
     gets zeros (``flash_attention``: NaN).  ``window >= Sk`` is plain causal attention.
-    A sequence's bits do not depend on the batch.
+    ``batch_invariant``: a sequence's bits do not depend on the batch (as in ``linear``).
     """
     what = "window_attention"
     index = _check_half(what, "q k v", q, k, v)
@@ -574,7 +576,7 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=Non
     b, h, sq, hd = q.shape
     _, hkv, sk, _ = k.shape
     if out is None:
-        out = torch.empty((b, sq, h * hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((b, sq, h * hd))
     else:
         _check_half(what, "q out", q, out)
         if tuple(out.shape) != (b, sq, h * hd):
@@ -587,10 +589,14 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=Non
         if kv.get_device() != index:
             raise ValueError(f"{what}: key_valid is on {kv.device}, not {q.device}")
     o_strides = _strides_array((b, h, sq), (out.stride(0), hd, out.stride(1)), 3)
+    invariant = int(bool(batch_invariant))
+    size = _bytes("tk_window_attn_workspace", b, h, hkv, sq, sk, hd, int(window), int(sinks), invariant)
+    ws = q.new_empty(size // 2) if size else None
     _launch_on(
         index, "window_attn", "tk_window_attn", q.data_ptr(), _strides_of(q, 3), k.data_ptr(), _strides_of(k, 3),
         v.data_ptr(), _strides_of(v, 3), out.data_ptr(), o_strides, _HALF_CODE[q.dtype], b, h, hkv, sq, sk, hd,
-        float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk,
+        float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk, invariant,
+        ws.data_ptr() if size else None, size,
     )
     return out
 
@@ -621,7 +627,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
         raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
     lens = _check_int32(what, "lengths", lengths, index, b)
     if out is None:
-        out = torch.empty((b, h * hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((b, h * hd))
     else:
         _check_half(what, "q out", q, out)
         if tuple(out.shape) != (b, h * hd):
@@ -629,7 +635,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
     most = width * page_size if max_length is None or batch_invariant else int(max_length)
     plan = (int(window), int(sinks), int(bool(batch_invariant)))
     size = _bytes("tk_paged_attn_workspace", b, h, hkv, hd, most, *plan)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    ws = q.new_empty(size // 2) if size else None
     _launch_on(
         index, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_of(q, 2), k_pages.data_ptr(),
         _strides_of(k_pages, 3), v_pages.data_ptr(), _strides_of(v_pages, 3), out.data_ptr(),
@@ -682,7 +688,7 @@ def cache_reserve(table, lengths, refs, new, page_size: int):
     state = _state_args(what, table, lengths, refs, page_size)
     index, rows = table.get_device(), state[3]
     added = _check_int32(what, "new", new, index, rows)
-    status, ws, size = _plan_buffers(table.device, rows, refs.shape[0])
+    status, ws, size = _plan_buffers(table, rows, refs.shape[0])
     _launch_on(index, "cache_reserve", "tk_cache_reserve", *state, added, status.data_ptr(),
                ws.data_ptr(), size)
     return status
@@ -706,7 +712,7 @@ def cache_fork(k_pages, v_pages, table, lengths, refs, parents, children):
     first = _check_int32(what, "parents", parents, index)
     n = parents.shape[0]
     second = _check_int32(what, "children", children, index, n)
-    status, ws, size = _plan_buffers(table.device, state[3], refs.shape[0], n)
+    status, ws, size = _plan_buffers(table, state[3], refs.shape[0], n)
     _launch_on(index, "cache_fork", "tk_cache_fork", *cache, *state, first, second, n, status.data_ptr(),
                ws.data_ptr(), size)
     return status
@@ -734,7 +740,7 @@ def cache_compact(k_pages, v_pages, table, lengths, refs):
     what = "cache_compact"
     cache = _cache_args(what, k_pages, v_pages, refs)
     state = _state_args(what, table, lengths, refs, k_pages.shape[-2])
-    used, ws, size = _plan_buffers(table.device, state[3], refs.shape[0])
+    used, ws, size = _plan_buffers(table, state[3], refs.shape[0])
     _launch_on(table.get_device(), "cache_compact", "tk_cache_compact", *cache, *state, used.data_ptr(),
                ws.data_ptr(), size)
     return used
