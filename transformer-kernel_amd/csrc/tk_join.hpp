@@ -1,8 +1,8 @@
 // Attention whose keys are split over workgroups: what they leave behind, and the launch that joins it.
 //
-// A row is one query of one head.  Split s of row r leaves its unnormalised output O (fp32, hd
-// values) relative to its running maximum m (in units of log2), and {m, sum of weights}; a split
-// that saw no key leaves m = -inf and no O.  The row is sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s
+// A row is one query of one head.  Split s of row r leaves, in a slot of its own, its unnormalised
+// output O (fp32, hd values) relative to its running maximum m (in units of log2), and
+// {m, sum of weights}; a split that saw no key leaves m = -inf and no O.  The row is sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s
 // with m the largest m_s, and zeros where nothing was seen.
 #pragma once
 #include "tk_elem.hpp"
@@ -11,75 +11,92 @@ namespace tk {
 namespace {
 
 struct JoinArgs {
-  const float* part;   // [rows][splits][hd]
-  const float* stats;  // [rows][splits][2]
+  const float* part;   // [slots][hd]
+  const float* stats;  // [slots][2]
   void* o;
-  int64_t os[3];  // elements, {b, h, s}
-  int heads, q_len, hd, splits;
-  int cols;  // columns of a row that a workgroup joins
+  // Nullable: {first slot w, splits} of each sequence.  Split s of a row lies in slot (w + s) * heads + h; one
+  // split alone is the output already.  Without a plan row r's splits lie in slots r * splits + s.
+  const int32_t* plan;
+  int64_t os[3];        // elements, {b, h, s}
+  int heads, q_len, hd;
+  int splits;  // without a plan: of every row; with one: about how many
+  int64_t rows;
 };
 
-constexpr int kJoin = 256;
+constexpr int kJoinWaves = 4;
 
-// Workgroups of kJoin / lpr groups of lpr lanes with 4 columns each, group i taking splits i, i + groups,
-// ...; the groups are added in their order, so the sums have one order whatever the batch.  (One wave that
-// walked 391 splits of a row of 128 alone took 235 us, 16 groups of one workgroup 16 us.)
-template <typename T>
-__global__ __launch_bounds__(kJoin) void split_join_kernel(JoinArgs p) {
-  __shared__ float m_lds[kJoin / 64];
-  __shared__ f32x4 o_lds[kJoin];
-  __shared__ float l_lds[kJoin];
-  const int blocks = (p.hd + p.cols - 1) / p.cols;
-  const int64_t rowid = blockIdx.x / blocks;
-  const float* st = p.stats + 2 * rowid * p.splits;
-  float m = -INFINITY;
-  for (int s = threadIdx.x; s < p.splits; s += kJoin) m = fmaxf(m, st[2 * s]);
-  m = group_max<64>(m);
-  if ((threadIdx.x & 63) == 0) m_lds[threadIdx.x >> 6] = m;
-  __syncthreads();
+// A result in the making: maximum, sum of weights and 4 columns of O relative to the maximum.
+struct JoinPart {
+  float m, l;
+  f32x4 o;
+  __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+    m = top;
+    l = f * l + f2 * l2;
 #pragma unroll
-  for (int w = 0; w < kJoin / 64; ++w) m = fmaxf(m, m_lds[w]);
-  const float m_ref = m == -INFINITY ? 0.f : m;
+    for (int e = 0; e < 4; ++e) o[e] = f * o[e] + f2 * o2[e];
+  }
+};
 
-  const int lpr = p.cols / 4, groups = kJoin / lpr;
-  const int grp = threadIdx.x / lpr, d = (int)(blockIdx.x % blocks) * p.cols + (threadIdx.x % lpr) * 4;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  if (d < p.hd) {
-    const float* part = p.part + rowid * p.splits * p.hd + d;
-#pragma unroll 4
-    for (int s = grp; s < p.splits; s += groups) {
-      if (st[2 * s] == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(st[2 * s] - m_ref);
-      const f32x4 o = *reinterpret_cast<const f32x4*>(part + (int64_t)s * p.hd);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, o[e], sum[e]);
-      l = fmaf(f, st[2 * s + 1], l);
-    }
-  }
-  o_lds[threadIdx.x] = sum;
-  l_lds[threadIdx.x] = l;
-  __syncthreads();
-  if (grp != 0 || d >= p.hd) return;
-  for (int i = 1; i < min(groups, p.splits); ++i) {
-    const f32x4 o = o_lds[i * lpr + threadIdx.x];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += o[e];
-    l += l_lds[i * lpr + threadIdx.x];
-  }
+// GROUPED: a workgroup joins 16 columns of a row, with 64 groups of 4 lanes; else a wave joins a row, with
+// groups of 16, 32 or 64 lanes.  Group i takes splits i, i + groups, ..., and the groups are merged as one
+// tree, so the sums have one order whatever the batch.  A chain of load latencies (the plan, the results),
+// so nothing waits for the maximum of all splits: 256 splits of 16 rows of 128 take 4.3 us, 2 of 1024 rows
+// 3.5.
+template <typename T, bool GROUPED>
+__global__ __launch_bounds__(kJoinWaves * 64) void split_join_kernel(JoinArgs p) {
+  __shared__ JoinPart lds[GROUPED ? kJoinWaves : 1][4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int blocks = GROUPED ? (p.hd + 15) / 16 : 1;
+  const int64_t rowid = GROUPED ? blockIdx.x / blocks : (int64_t)blockIdx.x * kJoinWaves + wave;
+  if (rowid >= p.rows) return;
   const int64_t bh = rowid / p.q_len;
-  T* out = reinterpret_cast<T*>(p.o) + bh / p.heads * p.os[0] + bh % p.heads * p.os[1] + rowid % p.q_len * p.os[2] + d;
+  const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
+  const int splits = p.plan ? p.plan[2 * b + 1] : p.splits;
+  if (p.plan && splits == 1) return;
+  const int64_t base = p.plan ? (int64_t)p.plan[2 * b] * p.heads + h : rowid * p.splits;
+  const int64_t step = p.plan ? p.heads : 1;
+  const int lpr = GROUPED ? 4 : p.hd <= 64 ? 16 : p.hd <= 128 ? 32 : 64;
+  const int groups = (GROUPED ? kJoinWaves * 64 : 64) / lpr, grp = (GROUPED ? (int)threadIdx.x : lane) / lpr;
+  const int d = (GROUPED ? (int)(blockIdx.x % blocks) * 16 : 0) + lane % lpr * 4, dc = min(d, p.hd - 4);
+
+  JoinPart r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 4
+  for (int s = grp; s < splits; s += groups) {
+    const int64_t at = base + s * step;
+    const f32x2 st = *reinterpret_cast<const f32x2*>(p.stats + 2 * at);
+    f32x4 o = *reinterpret_cast<const f32x4*>(p.part + at * p.hd + dc);
+    if (st[0] == -INFINITY) o = f32x4{0.f, 0.f, 0.f, 0.f};  // an empty split wrote no O
+    r.add(st[0], st[1], o);
+  }
+  for (int off = lpr; off < 64; off <<= 1) {
+    f32x4 o;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.f ? 0.f : sum[e] / l);
+    for (int e = 0; e < 4; ++e) o[e] = __shfl_xor(r.o[e], off);
+    r.add(__shfl_xor(r.m, off), __shfl_xor(r.l, off), o);
+  }
+  if constexpr (GROUPED) {
+    if (lane < 4) lds[wave][lane] = r;
+    __syncthreads();
+    if (threadIdx.x >= 4) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) r.add(lds[w][lane].m, lds[w][lane].l, lds[w][lane].o);
+  }
+  if (lane >= lpr || d >= p.hd) return;
+  T* out = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + rowid % p.q_len * p.os[2] + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(r.l == 0.f ? 0.f : r.o[e] / r.l);
 }
 
 template <typename T>
-int launch_join(const char* fn, JoinArgs p, int64_t rows, hipStream_t st) {
-  // many splits: 16 columns to a workgroup, so that 64 groups share them; few: a row to a workgroup
-  p.cols = p.splits > 32 ? 16 : p.hd <= 64 ? 64 : p.hd <= 128 ? 128 : 256;
-  const int64_t grid = rows * ((p.hd + p.cols - 1) / p.cols);
+int launch_join(const char* fn, const JoinArgs& p, hipStream_t st) {
+  const bool grouped = p.splits > 16;
+  const int64_t grid = grouped ? p.rows * ((p.hd + 15) / 16) : (p.rows + kJoinWaves - 1) / kJoinWaves;
   TK_REQUIRE(grid < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
-  hipLaunchKernelGGL((split_join_kernel<T>), dim3((unsigned)grid), dim3(kJoin), 0, st, p);
+  const dim3 g((unsigned)grid), blk(kJoinWaves * 64);
+  if (grouped) hipLaunchKernelGGL((split_join_kernel<T, true>), g, blk, 0, st, p);
+  else hipLaunchKernelGGL((split_join_kernel<T, false>), g, blk, 0, st, p);
   return check_launch(fn);
 }
 

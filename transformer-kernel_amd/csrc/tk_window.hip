@@ -521,7 +521,8 @@ int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   j.q_len = p.q_len;
   j.hd = p.hd;
   j.splits = p.splits;
-  return launch_join<T>(fn, j, (int64_t)p.batch * p.heads * p.q_len, st);
+  j.rows = (int64_t)p.batch * p.heads * p.q_len;
+  return launch_join<T>(fn, j, st);
 }
 
 template <typename T>
