@@ -176,7 +176,9 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
     // nothing of this tile for any of the wave's rows
     if (k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
 
+    // the products ahead of another wave's exponentials: 588 -> 568 us at head_dim 128
     f32x16 s[NB];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
@@ -184,6 +186,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
         const x8 kf = *reinterpret_cast<const x8*>(ks_ + swz_off<RB>(kb2 * 32 + (lane & 31), 2 * kk + g));
         s[kb2] = Elem<T>::mfma32(kf, qf[kk], kk == 0 ? f32x16{} : s[kb2]);
       }
+    __builtin_amdgcn_s_setprio(0);
     const bool whole = k0 + BN - 1 <= w_lo && (k0 > w_hi - p.window || k0 + BN <= p.sinks);
     if (KMASK || !whole) {
       const uint64_t kbits = bits >> (4 * g);
@@ -269,7 +272,10 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
-  int id = blockIdx.x;
+  // as in window_body, an XCD takes neighbouring blocks
+  const int total = p.n_qt * p.batch * p.heads * p.splits, per = (total + 7) / 8;
+  int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (id >= total) return;
   const int split = id % p.splits;
   id /= p.splits;
   const int qt = id % p.n_qt, bh = id / p.n_qt;
@@ -472,7 +478,7 @@ __global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_attn_kernel
   window_body<T, DT, BN, NW, KMASK>(p);
 }
 
-constexpr int kSplitWaves = 4;
+constexpr int kWindowWaves = 4;
 
 // Which kernel, and over how many workgroups window_split_kernel deals a block of 32 rows' keys.
 struct WindowPlan {
@@ -488,28 +494,27 @@ WindowPlan window_plan(int64_t bh, int64_t q_len, int64_t k_len, int64_t window,
   const int64_t tiles = (keys + bn - 1) / bn + 2;  // the sinks and the windows may begin and end inside tiles
   const int64_t want = (512 + bh * ((q_len + 31) / 32) - 1) / (bh * ((q_len + 31) / 32));
   int64_t per = (tiles + want - 1) / want;
-  per = (per + kSplitWaves - 1) / kSplitWaves * kSplitWaves;
-  if (per < 2 * kSplitWaves) per = 2 * kSplitWaves;
+  per = (per + kWindowWaves - 1) / kWindowWaves * kWindowWaves;
+  if (per < 2 * kWindowWaves) per = 2 * kWindowWaves;
   return {true, (tiles + per - 1) / per, per};
 }
 
 template <typename T, int DT, int BN, int BNS>
 int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
-  constexpr int NW = 4;
+  constexpr int NW = kWindowWaves;
   const char* fn = "tk_window_attn";
   const int rows = plan.split ? 32 : 32 * NW;
   p.n_qt = (p.q_len + rows - 1) / rows;
   const int64_t total = (int64_t)p.n_qt * p.batch * p.heads * plan.splits;
   TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
   if (!plan.split) {
-    const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
     if (p.kv) hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, true>), g, blk, 0, st, p);
     else hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, false>), g, blk, 0, st, p);
     return check_launch(fn);
   }
-  const dim3 g((unsigned)total), blk(kSplitWaves * 64);
-  if (p.kv) hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kSplitWaves, true>), g, blk, 0, st, p);
-  else hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kSplitWaves, false>), g, blk, 0, st, p);
+  if (p.kv) hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kWindowWaves, true>), g, blk, 0, st, p);
+  else hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kWindowWaves, false>), g, blk, 0, st, p);
   const int rc = check_launch(fn);
   if (rc != TK_OK || p.splits == 1) return rc;
   JoinArgs j{};
