@@ -535,7 +535,8 @@ int tk_cache_append(const void *k, const int64_t *k_strides, const void *v,
  * reserve: lengths[b] += added[b] >= 0 for every row, with the pages that this needs.
  * fork:    child i (an empty row, named once) becomes a copy of parent i as it was before the
  *          call: it shares the parent's whole pages and gets a page of its own with the rows
- *          of the one that is begun, in every layer (strides {layer, page, head, row}).
+ *          of the one that is begun, in every layer (strides {layer, page, head, row}).  At most
+ *          2^18 rows.
  * free:    every listed row gives up its pages (-1 in the table) and has length 0; rows that
  *          are not in the table are passed over, a row listed twice is freed once.
  * compact: with `used` live pages in all, the i-th live page of those with id >= used moves

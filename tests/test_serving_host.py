@@ -94,7 +94,7 @@ def test_cache_calls_refuse():
     def reserve(new=16, status=16, ws=16, size=1 << 20, **kw):
         return lib.tk_cache_reserve(*state(**kw), new, status, ws, size, None)
 
-    for call, code in [(dict(new=None), -1), (dict(status=None), -1), (dict(ws=None), -1), (dict(size=39), -1),
+    for call, code in [(dict(new=None), -1), (dict(status=None), -1), (dict(ws=None), -1), (dict(size=31), -1),
                        (dict(ps=0), -2), (dict(refs=None), -1), (dict(lengths=None), -1), (dict(stride=2), -1),
                        (dict(rows=-1), -1), (dict(pages=-1), -1)]:
         assert reserve(**call) == code, call
@@ -105,18 +105,19 @@ def test_cache_calls_refuse():
     def fork(parents=16, children=16, n=1, status=16, ws=16, size=1 << 20, cache=pages_args(), **kw):
         return lib.tk_cache_fork(*cache, *state(**kw), parents, children, n, status, ws, size, None)
 
-    for call, code in [(dict(parents=None), -1), (dict(n=-1), -1), (dict(status=None), -1), (dict(size=50), -1),
+    for call, code in [(dict(parents=None), -1), (dict(n=-1), -1), (dict(status=None), -1), (dict(size=39), -1),
                        (dict(cache=pages_args(k=None)), -1), (dict(cache=pages_args(k=8)), -2),
                        (dict(cache=pages_args(hd=4)), -2), (dict(cache=pages_args(layers=-1)), -1),
                        (dict(cache=pages_args(strides=_lib.strides([1, 64, 64, 64]))), -2),
-                       (dict(cache=pages_args(hkv=65535, hd=256), ps=1024), -1), (dict(width=-1), -1)]:
+                       (dict(cache=pages_args(hkv=65535, hd=256), ps=1024), -1), (dict(width=-1), -1),
+                       (dict(rows=(1 << 18) + 1, width=1, stride=1), -2)]:
         assert fork(**call) == code, call
     assert lib.tk_cache_free(*state(), None, 1, None) == -1
     assert lib.tk_cache_free(*state(), 16, -1, None) == -1
     assert lib.tk_cache_free(*state(), None, 0, None) == 0
     assert lib.tk_cache_compact(*pages_args(), *state(), None, 16, 1 << 20, None) == -1
     assert lib.tk_cache_compact(*pages_args(), *state(), 16, 16, 4 * 16, None) == -1
-    assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (2 + 9 + 16)
+    assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (6 + 16)
 
 
 def test_wrappers_refuse_on_the_cpu():

@@ -76,9 +76,12 @@ struct CacheArgs {
   int32_t* work;
 };
 
+constexpr int kFresh = 4096;  // new pages that a plan keeps in LDS; more go through its workspace
+
 struct PlanLds {
   int wave[kPlanWaves];
   int flag;
+  int32_t fresh[kFresh];
 };
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
@@ -107,18 +110,25 @@ __device__ __forceinline__ int plan_scan(int x, PlanLds& lds, int& total) {
   return before + incl - x;
 }
 
+// A step's refs: thread (wave, lane) holds those of pages base + 512 wave + 64 j + lane.
+typedef int PlanRefs[kScan];
+__device__ __forceinline__ void load_refs(const int32_t* refs, int pages, int base, PlanRefs& r) {
+  const int at = base + (int)(threadIdx.x >> 6) * 64 * kScan + (int)(threadIdx.x & 63);
+#pragma unroll
+  for (int j = 0; j < kScan; ++j) r[j] = at + 64 * j < pages ? refs[at + 64 * j] : 0;
+}
+
 // The pages that `take(page, refs)` picks, in ascending order, into list; stops after a step in
-// which `want` were reached.  Returns how many were found (at least min(want, all)).
+// which `want` were reached.  Returns how many were found (at least min(want, all)).  r: the first
+// step's refs, which the caller loads ahead of what it does before (their latency is 2 us on a chip whose
+// other XCDs wrote them last).
 template <typename Take>
 __device__ __forceinline__ int plan_collect(const int32_t* refs, int pages, int want, int32_t* list, int room,
-                                            PlanLds& lds, Take take) {
+                                            PlanLds& lds, PlanRefs& r, Take take) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int found = 0;
   for (int base = 0; base < pages && found < want; base += kPlan * kScan) {
     const int at = base + wave * 64 * kScan + lane;
-    int r[kScan];
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) r[j] = at + 64 * j < pages ? refs[at + 64 * j] : 0;
     uint64_t mask[kScan];
     int mine = 0;
 #pragma unroll
@@ -126,6 +136,7 @@ __device__ __forceinline__ int plan_collect(const int32_t* refs, int pages, int 
       mask[j] = __ballot(at + 64 * j < pages && take(at + 64 * j, r[j]));
       mine += __popcll(mask[j]);
     }
+    if (base + kPlan * kScan < pages) load_refs(refs, pages, base + kPlan * kScan, r);
     if (lane == 0) lds.wave[wave] = mine;
     __syncthreads();
     int rank = found;
@@ -148,56 +159,71 @@ __device__ __forceinline__ int plan_collect(const int32_t* refs, int pages, int 
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
 
-// work: [rows] first new page of each row, then [pages] free pages.
+// What row b needs, and where its new pages start in the list of all.
+struct ReserveRow {
+  int have, need, from, len;  // len: the new length, or -1
+};
+__device__ __forceinline__ ReserveRow reserve_row(const CacheArgs& p, int b, int before, PlanLds& lds, int& total) {
+  const int most = p.table_width << p.page_shift;
+  ReserveRow r = {0, 0, 0, 0};
+  if (b < p.rows) {
+    const int len = p.lengths[b], add = p.first[b];
+    if (len < 0 || add < 0 || len > most || add > most - len) {
+      lds.flag = 1;
+    } else {
+      r.have = pages_of(len, p.page_shift);
+      r.need = pages_of(len + add, p.page_shift) - r.have;
+      r.len = len + add;
+    }
+  }
+  r.from = before + plan_scan(r.need, lds, total);
+  return r;
+}
+
+// work: [pages] free pages.
 __device__ __forceinline__ void reserve_body(const CacheArgs& p) {
   __shared__ PlanLds lds;
   const int lane = threadIdx.x & 63;
-  const int most = p.table_width << p.page_shift;
-  int32_t* start = p.work;
-  int32_t* fresh = p.work + p.rows;
+  PlanRefs refs;
+  load_refs(p.refs, p.pages, 0, refs);
   if (threadIdx.x == 0) lds.flag = 0;
   __syncthreads();
   int total = 0;
+  ReserveRow row = {};  // of the last step: with up to kPlan rows it need not be found again
   for (int base = 0; base < p.rows; base += kPlan) {
-    const int b = base + (int)threadIdx.x;
-    int need = 0;
-    if (b < p.rows) {
-      const int len = p.lengths[b], add = p.first[b];
-      if (len < 0 || add < 0 || len > most || add > most - len) lds.flag = 1;
-      else need = pages_of(len + add, p.page_shift) - pages_of(len, p.page_shift);
-    }
     int sum;
-    const int before = plan_scan(need, lds, sum);
-    if (b < p.rows) start[b] = total + before;
+    row = reserve_row(p, base + (int)threadIdx.x, total, lds, sum);
     total += sum;
   }
-  __syncthreads();
   if (lds.flag) {
     if (threadIdx.x == 0) *p.status = kBadRows;
     return;
   }
-  const int found = plan_collect(p.refs, p.pages, total, fresh, p.pages, lds, [](int, int r) { return r <= 0; });
+  int32_t* fresh = total <= kFresh ? lds.fresh : p.work;
+  const int found = plan_collect(p.refs, p.pages, total, fresh, total, lds, refs,
+                                 [](int, int r) { return r <= 0; });
   if (threadIdx.x == 0) *p.status = max(0, total - found);
   if (found < total) return;
+  int before = 0;
   for (int base = 0; base < p.rows; base += kPlan) {
     const int b = base + (int)threadIdx.x;
-    int have = 0, need = 0, from = 0;
+    if (p.rows > kPlan) {
+      int sum;
+      row = reserve_row(p, b, before, lds, sum);
+      before += sum;
+    }
     if (b < p.rows) {
-      const int len = p.lengths[b], add = p.first[b];
-      have = pages_of(len, p.page_shift);
-      need = pages_of(len + add, p.page_shift) - have;
-      from = start[b];
-      p.lengths[b] = len + add;
-      if (need == 1) {
-        const int page = fresh[from];
-        p.table[b * p.table_stride + have] = page;
+      p.lengths[b] = row.len;
+      if (row.need == 1) {
+        const int page = fresh[row.from];
+        p.table[b * p.table_stride + row.have] = page;
         p.refs[page] = 1;
       }
     }
     // rows that need more (a prompt's): the whole wave for each
-    for (uint64_t many = __ballot(need > 1); many; many &= many - 1) {
+    for (uint64_t many = __ballot(row.need > 1); many; many &= many - 1) {
       const int src = __builtin_ctzll(many);
-      const int rb = __shfl(b, src), rh = __shfl(have, src), rn = __shfl(need, src), rf = __shfl(from, src);
+      const int rb = __shfl(b, src), rh = __shfl(row.have, src), rn = __shfl(row.need, src), rf = __shfl(row.from, src);
       for (int i = lane; i < rn; i += 64) {
         const int page = fresh[rf + i];
         p.table[rb * p.table_stride + rh + i] = page;
@@ -209,57 +235,59 @@ __device__ __forceinline__ void reserve_body(const CacheArgs& p) {
 
 __global__ __launch_bounds__(kPlan) void cache_reserve_kernel(CacheArgs p) { reserve_body(p); }
 
-// work: [rows] times a row is a child, [n] parents' lengths, [n] fresh pages, [n] pages they are
-// copied from, then [pages] free pages.
+// work: [n] parents' lengths, [n] fresh pages, then [pages] free pages.
 struct ForkWork {
-  int32_t *seen, *len, *fresh, *src, *free;
+  int32_t *len, *fresh, *free;
 };
 __device__ __forceinline__ ForkWork fork_work(const CacheArgs& p) {
-  return {p.work, p.work + p.rows, p.work + p.rows + p.n, p.work + p.rows + 2 * (int64_t)p.n,
-          p.work + p.rows + 3 * (int64_t)p.n};
+  return {p.work, p.work + p.n, p.work + 2 * (int64_t)p.n};
 }
+
+constexpr int kForkRows = 1 << 18;  // rows of a table that forks: a bit each in LDS
 
 __device__ __forceinline__ void fork_plan_body(const CacheArgs& p) {
   __shared__ PlanLds lds;
+  __shared__ uint32_t seen[kForkRows / 32];  // rows that are children already
   const ForkWork w = fork_work(p);
   const int most = p.table_width << p.page_shift;
+  PlanRefs refs;
+  load_refs(p.refs, p.pages, 0, refs);
   if (threadIdx.x == 0) lds.flag = 0;
-  for (int b = threadIdx.x; b < p.rows; b += kPlan) w.seen[b] = 0;
-  __threadfence();
+  for (int i = threadIdx.x; i < (p.rows + 31) / 32; i += kPlan) seen[i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < p.n; i += kPlan) {
-    const int child = p.second[i];
-    if ((uint32_t)child >= (uint32_t)p.rows || atomicAdd(&w.seen[child], 1) != 0) lds.flag = 1;
-  }
-  int total = 0;
+  int total = 0, rank = -1;  // rank of the last step: with up to kPlan children it need not be kept
   for (int base = 0; base < p.n; base += kPlan) {
     const int i = base + (int)threadIdx.x;
     int need = 0;
     if (i < p.n) {
       const int parent = p.first[i], child = p.second[i];
       int len = -1;
-      if ((uint32_t)parent < (uint32_t)p.rows && (uint32_t)child < (uint32_t)p.rows && p.lengths[child] == 0)
+      if ((uint32_t)parent < (uint32_t)p.rows && (uint32_t)child < (uint32_t)p.rows && p.lengths[child] == 0 &&
+          !((atomicOr(&seen[child >> 5], 1u << (child & 31)) >> (child & 31)) & 1))
         len = p.lengths[parent];
       if (len < 0 || len > most) lds.flag = 1;
       else need = (len & ((1 << p.page_shift) - 1)) != 0;
       w.len[i] = len;
-      w.src[i] = need ? p.table[parent * p.table_stride + (len >> p.page_shift)] : -1;
     }
     int sum;
     const int before = plan_scan(need, lds, sum);
-    if (i < p.n) w.fresh[i] = need ? total + before : -1;
+    rank = need ? total + before : -1;
+    if (i < p.n && p.n > kPlan) w.fresh[i] = rank;
     total += sum;
   }
-  __syncthreads();
   if (lds.flag) {
     if (threadIdx.x == 0) *p.status = kBadRows;
     return;
   }
-  const int found = plan_collect(p.refs, p.pages, total, w.free, p.pages, lds, [](int, int r) { return r <= 0; });
+  int32_t* fresh = total <= kFresh ? lds.fresh : w.free;
+  const int found = plan_collect(p.refs, p.pages, total, fresh, total, lds, refs,
+                                 [](int, int r) { return r <= 0; });
   if (threadIdx.x == 0) *p.status = max(0, total - found);
   if (found < total) return;
-  for (int i = threadIdx.x; i < p.n; i += kPlan)
-    if (w.fresh[i] >= 0) w.fresh[i] = w.free[w.fresh[i]];
+  for (int i = threadIdx.x; i < p.n; i += kPlan) {
+    if (p.n > kPlan) rank = w.fresh[i];
+    w.fresh[i] = rank >= 0 ? fresh[rank] : -1;
+  }
 }
 
 __global__ __launch_bounds__(kPlan) void cache_fork_plan_kernel(CacheArgs p) { fork_plan_body(p); }
@@ -288,8 +316,9 @@ __global__ __launch_bounds__(256) void cache_fork_kernel(CacheArgs p) {
     }
     return;
   }
-  const int src = w.src[i];
-  if (fresh < 0 || (uint32_t)src >= (uint32_t)p.pages) return;
+  if (fresh < 0) return;  // (a parent is no child but of an empty row: its entries stand)
+  const int src = p.table[p.first[i] * p.table_stride + whole];
+  if ((uint32_t)src >= (uint32_t)p.pages) return;
   const int l = (part - 1) / p.kv_heads, h = (part - 1) % p.kv_heads;
   const int items = (len & ((1 << p.page_shift) - 1)) * p.vecs;
   const int64_t kb = l * p.ks[0] + h * p.ks[2], vb = l * p.vs[0] + h * p.vs[2];
@@ -325,11 +354,16 @@ __device__ __forceinline__ void compact_plan_body(const CacheArgs& p) {
   int32_t* list = p.work + 1;
   int32_t* to = list + p.pages;
   int live = 0;
-  for (int i = threadIdx.x; i < p.pages; i += kPlan) live += p.refs[i] > 0;
+  PlanRefs refs;
+  for (int base = (p.pages - 1) / (kPlan * kScan) * (kPlan * kScan); base >= 0; base -= kPlan * kScan) {  // ends with step 0
+    load_refs(p.refs, p.pages, base, refs);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) live += refs[j] > 0;
+  }
   int used;
   plan_scan(live, lds, used);
   for (int i = used + (int)threadIdx.x; i < p.pages; i += kPlan) to[i] = i;
-  const int found = plan_collect(p.refs, p.pages, 0x7fffffff, list, p.pages, lds,
+  const int found = plan_collect(p.refs, p.pages, 0x7fffffff, list, p.pages, lds, refs,
                                  [used](int page, int r) { return page < used ? r <= 0 : r > 0; });
   const int m = found / 2;  // as many holes below `used` as live pages above
   for (int i = threadIdx.x; i < m; i += kPlan) {
@@ -479,7 +513,7 @@ using namespace tk;
 extern "C" int64_t tk_cache_workspace(int64_t rows, int64_t pages, int64_t n) {
   TK_REQUIRE(rows >= 0 && pages >= 0 && n >= 0 && rows < (1ll << 24) && pages < (1ll << 30) && n < (1ll << 24),
              TK_ERR_ARG, "tk_cache_workspace: size out of range");
-  return 4 * (rows + 3 * n + 2 * pages + 1);
+  return 4 * (2 * n + 2 * pages + 1);
 }
 
 extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -534,7 +568,7 @@ extern "C" int tk_cache_reserve(int32_t* table, int64_t table_stride, int64_t ta
   int rc = fill_cache(fn, p, table, table_stride, table_width, rows, lengths, refs, pages, page_size);
   if (rc != TK_OK) return rc;
   TK_REQUIRE(status && (added || rows == 0), TK_ERR_ARG, "%s: null pointer", fn);
-  if ((rc = check_workspace(fn, workspace, workspace_bytes, 4 * (rows + pages))) != TK_OK) return rc;
+  if ((rc = check_workspace(fn, workspace, workspace_bytes, 4 * pages)) != TK_OK) return rc;
   p.first = added;
   p.status = status;
   p.work = (int32_t*)workspace;
@@ -554,7 +588,8 @@ extern "C" int tk_cache_fork(void* k_pages, const int64_t* k_strides, void* v_pa
   if ((rc = fill_pages(fn, p, k_pages, k_strides, v_pages, v_strides, layers, kv_heads, head_dim)) != TK_OK) return rc;
   TK_REQUIRE(n >= 0 && n < (1ll << 24) && status && (n == 0 || (parents && children)), TK_ERR_ARG,
              "%s: bad parents or children", fn);
-  if ((rc = check_workspace(fn, workspace, workspace_bytes, 4 * (rows + 3 * n + pages))) != TK_OK) return rc;
+  TK_REQUIRE(rows <= kForkRows, TK_ERR_UNSUPPORTED, "%s: a table of more than %d rows", fn, kForkRows);
+  if ((rc = check_workspace(fn, workspace, workspace_bytes, 4 * (2 * n + pages))) != TK_OK) return rc;
   const int64_t grid = n * (1 + (int64_t)p.layers * p.kv_heads);
   TK_REQUIRE(grid < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many children", fn);
   p.first = parents;

@@ -248,11 +248,16 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
 
 // The same rows' keys dealt to the waves of a workgroup (and to several workgroups): for launches with too
 // few query rows to fill the chip, whose workgroups of the kernel above would walk their tiles as one
-// serial chain each.  32 rows of one head per workgroup; wave w takes every NW-th of its tiles, into K and V
-// slots of its own, so the loop has no barrier: the next K is copied when the current one's products
-// are done, the next V after P.V.  At the end the waves' (max, sum, O) are merged in wave order.
-template <typename T, int DT, int BN, int NW, bool KMASK>
+// serial chain each.  32 rows of one head per workgroup; wave w takes every NW-th of its tiles of kSplitKeys
+// keys, into K and V slots of its own, so the loop has no barrier: the next K is copied when the current
+// one's products are done, the next V after P.V.  At the end the waves' (max, sum, O) are merged in wave
+// order.  Tiles of 32 keys leave room for two to six workgroups per CU: 16 heads of 64, 619 rows, window 126
+// 9.0 us, with tiles of 64 11.7.  (Two waves of rows per tile, tiles ahead in a second slot: 14.0, and 31 us
+// instead of 38 where a window of 2048 keys makes the chains long.)
+constexpr int kSplitKeys = 32;
+template <typename T, int DT, int NW, bool KMASK>
 __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
+  constexpr int BN = kSplitKeys;
   typedef typename Elem<T>::x8 x8;
   typedef typename Elem<T>::x4 x4;
   constexpr int NB = BN / 32;
@@ -468,9 +473,9 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
   }
 }
 
-template <typename T, int DT, int BN, int NW, bool KMASK>
+template <typename T, int DT, int NW, bool KMASK>
 __global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_split_kernel(WindowArgs p) {
-  window_split_body<T, DT, BN, NW, KMASK>(p);
+  window_split_body<T, DT, NW, KMASK>(p);
 }
 
 template <typename T, int DT, int BN, int NW, bool KMASK>
@@ -487,19 +492,23 @@ struct WindowPlan {
 };
 WindowPlan window_plan(int64_t bh, int64_t q_len, int64_t k_len, int64_t window, int64_t sinks, int64_t hd,
                        bool batch_invariant) {
-  if (batch_invariant || bh * ((q_len + 127) / 128) > 256) return {false, 1, 0};
-  const int64_t bn = hd <= 64 ? 64 : 32;
+  // Workgroups of 128 rows fill the chip from one per CU on (two at head_dim 256, one wave per SIMD).
+  if (batch_invariant || bh * ((q_len + 127) / 128) > (hd > 128 ? 512 : 256)) return {false, 1, 0};
   int64_t keys = window + 31 + sinks;
   if (keys > k_len) keys = k_len;
-  const int64_t tiles = (keys + bn - 1) / bn + 2;  // the sinks and the windows may begin and end inside tiles
-  const int64_t want = (512 + bh * ((q_len + 31) / 32) - 1) / (bh * ((q_len + 31) / 32));
+  // the sinks and the windows may begin and end inside tiles
+  const int64_t tiles = (keys + kSplitKeys - 1) / kSplitKeys + 2, blocks = bh * ((q_len + 31) / 32);
+  // A block's keys go to several workgroups only up to one workgroup per CU, in shares of three tiles a wave or
+  // more: past that the launch that joins them costs more (10 x 2 heads of 128, 735 rows: whole 20 us, in two
+  // 38; 3 heads of 64, 923 rows, window 2920: 18 us in eight shares, 34 whole).
+  const int64_t want = blocks < 256 ? 256 / blocks : 1;
   int64_t per = (tiles + want - 1) / want;
   per = (per + kWindowWaves - 1) / kWindowWaves * kWindowWaves;
-  if (per < 2 * kWindowWaves) per = 2 * kWindowWaves;
+  if (per < 3 * kWindowWaves) per = 3 * kWindowWaves;
   return {true, (tiles + per - 1) / per, per};
 }
 
-template <typename T, int DT, int BN, int BNS>
+template <typename T, int DT, int BN>
 int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   constexpr int NW = kWindowWaves;
   const char* fn = "tk_window_attn";
@@ -513,8 +522,8 @@ int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
     else hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, false>), g, blk, 0, st, p);
     return check_launch(fn);
   }
-  if (p.kv) hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kWindowWaves, true>), g, blk, 0, st, p);
-  else hipLaunchKernelGGL((window_split_kernel<T, DT, BNS, kWindowWaves, false>), g, blk, 0, st, p);
+  if (p.kv) hipLaunchKernelGGL((window_split_kernel<T, DT, kWindowWaves, true>), g, blk, 0, st, p);
+  else hipLaunchKernelGGL((window_split_kernel<T, DT, kWindowWaves, false>), g, blk, 0, st, p);
   const int rc = check_launch(fn);
   if (rc != TK_OK || p.splits == 1) return rc;
   JoinArgs j{};
@@ -532,10 +541,10 @@ int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
 
 template <typename T>
 int dispatch_window(const WindowArgs& p, const WindowPlan& plan, hipStream_t st) {
-  if (p.hd <= 32) return launch_window<T, 32, 64, 64>(p, plan, st);
-  if (p.hd <= 64) return launch_window<T, 64, 64, 64>(p, plan, st);
-  if (p.hd <= 128) return launch_window<T, 128, 64, 32>(p, plan, st);
-  return launch_window<T, 256, 32, 32>(p, plan, st);
+  if (p.hd <= 32) return launch_window<T, 32, 64>(p, plan, st);
+  if (p.hd <= 64) return launch_window<T, 64, 64>(p, plan, st);
+  if (p.hd <= 128) return launch_window<T, 128, 64>(p, plan, st);
+  return launch_window<T, 256, 32>(p, plan, st);
 }
 
 }  // namespace
