@@ -297,6 +297,17 @@ def test_paged_long_sequence_splits_and_joins():
             assert torch.equal(one[0], whole[n])
 
 
+@pytest.mark.parametrize("b,hkv,longest", [(130, 1, 9000), (70, 2, 9100), (1030, 1, 300), (300, 1, 8300)])
+def test_paged_many_sequences_of_which_some_are_long(b, hkv, longest):
+    """Enough sequences for every CU, and among them (first, in the middle, last) some far longer than the others."""
+    lengths = [(37 * i) % 61 for i in range(b)]
+    lengths[0], lengths[b // 2], lengths[-1] = longest, longest - 333, longest - 1
+    k, v, table, lens = _cache(lengths, hkv, 64, 64, BF16, seed=17)
+    q = seeded(b, 2 * hkv, 64, dtype=BF16, seed=18)
+    _check_paged(q, k, v, table, lens)
+    _check_paged(q, k, v, table, lens, window=8200, sinks=3)
+
+
 # ------------------------------------------------------------------- cache --
 
 

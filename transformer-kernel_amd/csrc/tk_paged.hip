@@ -47,6 +47,7 @@ struct PagedArgs {
   int window, sinks;  // window 0: all keys
   int workers;  // workgroups per key head and block of heads
   bool shared;  // paged_share; else one worker per sequence, or fixed ones
+  bool fill;    // paged_share: as many shares as there are workers
   int least;    // tiles of the smallest share
   int fixed;    // > 0: shares of this many tiles, workers / batch of them per sequence
   float scale_log2;
@@ -96,12 +97,13 @@ struct PagedShare {
 };
 
 // Sequences of different lengths are cut into shares of nearly one size, so that every CU has the same to
-// do: sequence b of n_b tiles into ceil(n_b / size) equal ones, size being the smallest (in steps of the
-// workgroup's waves) at which there are no more shares than workers.  With one workgroup per CU in all, any
-// share too many shares its CU: 12 sequences of 36254 tokens, 4 key heads of 128, in 240 workgroups take
-// 153 us, in 288 206.  Every wave finds its worker's place from all lengths, at most kShareRows of them, a
-// few registers.
-constexpr int kShareRows = 256;
+// do: sequence b of n_b tiles into ceil(n_b / size) equal ones.  With fewer sequences than CUs (p.fill) size
+// is the smallest (in steps of the workgroup's waves) at which there are no more shares than workers: with
+// one workgroup per CU in all, any share too many shares its CU (12 sequences of 36254 tokens, 4 key heads
+// of 128, in 240 workgroups take 153 us, in 288 206).  With more, only sequences of more than twice what
+// a CU has on average are cut, which otherwise end long after all the others.  Every wave finds its
+// worker's place from all lengths, at most kShareRows of them, a few registers.
+constexpr int kShareRows = 1024;
 template <int NW>
 __device__ __forceinline__ PagedShare paged_share(const PagedArgs& p, int worker) {
   constexpr int kPer = kShareRows / 64;
@@ -119,7 +121,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs& p, int worker
   total = wave_sum(total);
   // ceil(n_b / size) add up to less than total / size + batch
   int low = max(total / (p.workers * NW), p.least / NW), high = max(total / ((p.workers - p.batch) * NW) + 1, low);
-  while (low < high) {
+  while (p.fill && low < high) {
     const int mid = (low + high) / 2;
     int n = 0;
 #pragma unroll
@@ -436,9 +438,10 @@ constexpr int kPagedWaves = 4;
 // Workers per key head and block of 16 heads; the others: PagedArgs.
 struct PagedPlan {
   int64_t workers, fixed;
-  bool shared;
+  bool shared, fill;
 };
 constexpr int64_t kPagedBlocks = 256;             // one workgroup per CU
+constexpr int64_t kPagedLong = 256;               // tiles from which on one sequence may outlast all others
 constexpr int64_t kPagedLeast = 2 * kPagedWaves;  // tiles of the smallest share: two steps of every wave
 PagedPlan paged_plan(int64_t batch, int64_t per_seq, int64_t max_length, int64_t window, int64_t sinks,
                      bool batch_invariant) {
@@ -447,15 +450,20 @@ PagedPlan paged_plan(int64_t batch, int64_t per_seq, int64_t max_length, int64_t
   const int64_t tiles = (keys + 31) / 32 + (window > 0 ? 2 : 0);  // a window may begin and end inside tiles
   if (batch_invariant) {
     const int64_t per = 32, n = (tiles + per - 1) / per;
-    return {batch * (n > 1 ? n : 1), per, false};
+    return {batch * (n > 1 ? n : 1), per, false, false};
   }
   const int64_t most = (tiles + kPagedLeast - 1) / kPagedLeast;  // shares of the longest sequence
-  // From half the CUs on, a split gains less than the launch that joins it takes: 186 sequences of 676 to 917
+  // From half the CUs on, a split of every sequence gains less than the launch that joins it takes: 186 sequences of 676 to 917
   // tokens, one key head of 64, in whole ones 10.7 us, split 16.8; 17 sequences of 4000, 8 key heads of 128
   // 57 and 70.  (Below: 2 sequences of 2000 tokens, 2 key heads of 128, 10 us split, 17 whole.)
-  if (2 * batch * per_seq >= kPagedBlocks || most <= 1) return {batch, 0, false};
+  const int64_t whole = kPagedBlocks / 2 / per_seq;  // sequences
+  if (batch >= whole) {
+    if (tiles < kPagedLong || batch > kShareRows) return {batch, 0, false, false};
+    return {batch + (whole > 1 ? whole : 1), 0, true, false};
+  }
+  if (most <= 1) return {batch, 0, false, false};
   const int64_t full = kPagedBlocks / per_seq, workers = full < batch * (most + 1) ? full : batch * (most + 1);
-  return {workers > batch ? workers : batch, 0, workers > batch};
+  return {workers, 0, true, true};
 }
 
 template <typename T, int DT>
@@ -606,6 +614,7 @@ extern "C" int tk_paged_attn(const void* q, const int64_t* q_strides, const void
   p.sinks = (int)sinks;
   p.workers = (int)plan.workers;
   p.shared = plan.shared;
+  p.fill = plan.fill;
   p.least = (int)kPagedLeast;
   p.fixed = (int)plan.fixed;
   p.scale_log2 = scale * 1.4426950408889634f;

@@ -540,8 +540,9 @@ def _cache_args(what: str, k_pages, v_pages, refs) -> tuple:
     return k.data_ptr(), _strides_of(k, 4), v.data_ptr(), _strides_of(v, 4), layers, hkv, hd
 
 
+@functools.lru_cache(maxsize=4096)
 def _bytes(fn: str, *args) -> int:
-    """What a workspace function of the library answers, or its refusal raised."""
+    """What a workspace function of the library answers for these sizes, or its refusal raised."""
     size = getattr(_lib.load(), fn)(*args)
     if size < 0:
         raise _lib.TkError(fn, size, _lib.load().tk_last_error_string().decode())
