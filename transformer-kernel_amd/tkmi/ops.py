@@ -470,36 +470,33 @@ def _strides_array(shape, stride, dims: int) -> "ctypes.Array":
     return _lib.strides([st if n > 1 else 0 for n, st in zip(shape[:dims], stride)])
 
 
-def _strides_of(t: torch.Tensor, dims: int) -> "ctypes.Array":
-    return _strides_array(t.shape, t.stride(), dims)
-
-
-def _check_half(what: str, names: str, *tensors: torch.Tensor) -> int:
-    """One 16-bit dtype, one device, contiguous last dimensions; returns the device's index."""
+def _check_half(what: str, names: str, *tensors: torch.Tensor) -> tuple:
+    """One 16-bit dtype, one device, contiguous last dimensions; returns the device's index and the strides."""
     dtype, index = tensors[0].dtype, tensors[0].get_device()
+    strides = []
     if index >= 0 and dtype in _HALF_CODE:
         for t in tensors:
-            if t.dtype is not dtype or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            st = t.stride()
+            if t.dtype is not dtype or t.get_device() != index or not st or (st[-1] != 1 and t.shape[-1] > 1):
                 break
+            strides.append(st)
         else:
-            return index
+            return index, strides
     _require_cuda(*tensors)
     for name, t in zip(names.split(), tensors):
         if t.dtype not in _HALF_CODE or t.dtype != dtype:
             raise TypeError(f"{what}: {name} is {t.dtype}; expected one of float16 and bfloat16 for all")
         if t.get_device() != index:
             raise ValueError(f"{what}: {name} is on {t.device}, not {tensors[0].device}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{what}: {name} needs a contiguous head_dim")
-    raise AssertionError("unreachable")
+    raise ValueError(f"{what}: {', '.join(names.split())} need a contiguous head_dim")
 
 
 def _check_int32(what: str, name: str, t: torch.Tensor, index: int, entries: Optional[int] = None) -> int:
     """A contiguous int32 vector on device ``index``, of ``entries`` entries if given; returns its address."""
     if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise TypeError(f"{what}: {name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-    if entries is not None and t.shape[0] != entries:
-        raise ValueError(f"{what}: {name} must have {entries} entries, got {t.shape[0]}")
+    if entries is not None and t.numel() != entries:
+        raise ValueError(f"{what}: {name} must have {entries} entries, got {t.numel()}")
     if t.get_device() != index:
         _require_cuda(t)
         raise ValueError(f"{what}: {name} is on {t.device}, not cuda:{index}")
@@ -508,14 +505,15 @@ def _check_int32(what: str, name: str, t: torch.Tensor, index: int, entries: Opt
 
 def _check_table(what: str, table: torch.Tensor, index: int) -> tuple:
     """table [rows, entries] on device ``index``; returns (pointer, row stride, entries, rows)."""
-    if table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
+    shape, stride = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise TypeError(f"{what}: table must be int32 [rows, entries] with contiguous rows, got {table.dtype} "
-                        f"{tuple(table.shape)}")
+                        f"{tuple(shape)}")
     if table.get_device() != index or index < 0:
         _require_cuda(table)
         raise ValueError(f"{what}: table is on {table.device}, not cuda:{index}")
-    rows, width = table.shape
-    return table.data_ptr(), table.stride(0) if rows > 1 else width, width, rows
+    rows, width = shape
+    return table.data_ptr(), stride[0] if rows > 1 else width, width, rows
 
 
 def _state_args(what: str, table, lengths, refs, page_size: int) -> tuple:
@@ -528,16 +526,18 @@ def _state_args(what: str, table, lengths, refs, page_size: int) -> tuple:
 
 def _cache_args(what: str, k_pages, v_pages, refs) -> tuple:
     """Pages [layers, pages, kv_heads, page_size, head_dim], or of one layer without the first dimension."""
-    index = _check_half(what, "k_pages v_pages", k_pages, v_pages)
-    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+    index, (ks, vs) = _check_half(what, "k_pages v_pages", k_pages, v_pages)
+    shape = k_pages.shape
+    if shape != v_pages.shape or len(shape) not in (4, 5):
         raise ValueError(f"{what}: k_pages and v_pages must share one shape [layers, pages, kv_heads, page_size, "
-                         f"head_dim], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    k = k_pages if k_pages.dim() == 5 else k_pages[None]
-    v = v_pages if v_pages.dim() == 5 else v_pages[None]
-    layers, pages, hkv, _, hd = k.shape
-    if index != refs.get_device() or pages != refs.shape[0]:
-        raise ValueError(f"{what}: refs must have one entry per page ({pages}) on {k.device}")
-    return k.data_ptr(), _strides_of(k, 4), v.data_ptr(), _strides_of(v, 4), layers, hkv, hd
+                         f"head_dim], got {tuple(shape)} and {tuple(v_pages.shape)}")
+    if len(shape) == 4:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    layers, pages, hkv, _, hd = shape
+    if index != refs.get_device() or pages != refs.numel():
+        raise ValueError(f"{what}: refs must have one entry per page ({pages}) on {k_pages.device}")
+    return (k_pages.data_ptr(), _strides_array(shape, ks, 4), v_pages.data_ptr(), _strides_array(shape, vs, 4), layers,
+            hkv, hd)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -570,34 +570,35 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0, out=Non
     ``batch_invariant``: a sequence's bits do not depend on the batch (as in ``linear``).
     """
     what = "window_attention"
-    index = _check_half(what, "q k v", q, k, v)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{what}: q [B, H, Sq, hd] and k, v [B, Hkv, Sk, hd] expected, got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    b, h, sq, hd = q.shape
-    _, hkv, sk, _ = k.shape
+    index, (qst, kst, vst) = _check_half(what, "q k v", q, k, v)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
+        raise ValueError(f"{what}: q [B, H, Sq, hd] and k, v [B, Hkv, Sk, hd] expected, got {tuple(qs)}, {tuple(ks)}, "
+                         f"{tuple(v.shape)}")
+    b, h, sq, hd = qs
+    _, hkv, sk, _ = ks
     if out is None:
         out = q.new_empty((b, sq, h * hd))
+        ost = (sq * h * hd, h * hd)
     else:
-        _check_half(what, "q out", q, out)
-        if tuple(out.shape) != (b, sq, h * hd):
+        if out.shape != (b, sq, h * hd):
             raise ValueError(f"{what}: out must be [B, Sq, H*hd] = {(b, sq, h * hd)}, got {tuple(out.shape)}")
+        ost = _check_half(what, "q out", q, out)[1][1]
     kv = None
     if key_valid is not None:
-        if tuple(key_valid.shape) != (b, sk):
+        if key_valid.shape != (b, sk):
             raise ValueError(f"{what}: key_valid must be [B, Sk] = {(b, sk)}, got {tuple(key_valid.shape)}")
         kv = _row_mask(key_valid, b * sk)
         if kv.get_device() != index:
             raise ValueError(f"{what}: key_valid is on {kv.device}, not {q.device}")
-    o_strides = _strides_array((b, h, sq), (out.stride(0), hd, out.stride(1)), 3)
-    invariant = int(bool(batch_invariant))
-    size = _bytes("tk_window_attn_workspace", b, h, hkv, sq, sk, hd, int(window), int(sinks), invariant)
+    window, sinks, invariant = int(window), int(sinks), int(bool(batch_invariant))
+    size = _bytes("tk_window_attn_workspace", b, h, hkv, sq, sk, hd, window, sinks, invariant)
     ws = q.new_empty(size // 2) if size else None
     _launch_on(
-        index, "window_attn", "tk_window_attn", q.data_ptr(), _strides_of(q, 3), k.data_ptr(), _strides_of(k, 3),
-        v.data_ptr(), _strides_of(v, 3), out.data_ptr(), o_strides, _HALF_CODE[q.dtype], b, h, hkv, sq, sk, hd,
-        float(scale), int(window), int(sinks), kv.data_ptr() if kv is not None else None, sk, invariant,
-        ws.data_ptr() if size else None, size,
+        index, "window_attn", "tk_window_attn", q.data_ptr(), _strides_array(qs, qst, 3), k.data_ptr(),
+        _strides_array(ks, kst, 3), v.data_ptr(), _strides_array(ks, vst, 3), out.data_ptr(),
+        _strides_array((b, h, sq), (ost[0], hd, ost[1]), 3), _HALF_CODE[q.dtype], b, h, hkv, sq, sk, hd, float(scale),
+        window, sinks, kv.data_ptr() if kv is not None else None, sk, invariant, ws.data_ptr() if size else None, size,
     )
     return out
 
@@ -617,31 +618,33 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
     sequence's bits do not depend on the batch or ``max_length``.
     """
     what = "paged_attention"
-    index = _check_half(what, "q k_pages v_pages", q, k_pages, v_pages)
-    if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or q.shape[2] != k_pages.shape[3]:
-        raise ValueError(f"{what}: q [B, H, hd] and pages [pages, Hkv, page_size, hd] expected, got {tuple(q.shape)}, "
-                         f"{tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    b, h, hd = q.shape
-    pages, hkv, page_size, _ = k_pages.shape
+    index, (qst, kst, vst) = _check_half(what, "q k_pages v_pages", q, k_pages, v_pages)
+    qs, ks = q.shape, k_pages.shape
+    if len(qs) != 3 or len(ks) != 4 or ks != v_pages.shape or qs[2] != ks[3]:
+        raise ValueError(f"{what}: q [B, H, hd] and pages [pages, Hkv, page_size, hd] expected, got {tuple(qs)}, "
+                         f"{tuple(ks)}, {tuple(v_pages.shape)}")
+    b, h, hd = qs
+    pages, hkv, page_size, _ = ks
     ptr, stride, width, rows = _check_table(what, table, index)
     if rows != b:
         raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
     lens = _check_int32(what, "lengths", lengths, index, b)
     if out is None:
         out = q.new_empty((b, h * hd))
+        out_row = h * hd
     else:
-        _check_half(what, "q out", q, out)
-        if tuple(out.shape) != (b, h * hd):
+        if out.shape != (b, h * hd):
             raise ValueError(f"{what}: out must be [B, H*hd] = {(b, h * hd)}, got {tuple(out.shape)}")
+        out_row = _check_half(what, "q out", q, out)[1][1][0]
     most = width * page_size if max_length is None or batch_invariant else int(max_length)
     plan = (int(window), int(sinks), int(bool(batch_invariant)))
     size = _bytes("tk_paged_attn_workspace", b, h, hkv, hd, most, *plan)
     ws = q.new_empty(size // 2) if size else None
     _launch_on(
-        index, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_of(q, 2), k_pages.data_ptr(),
-        _strides_of(k_pages, 3), v_pages.data_ptr(), _strides_of(v_pages, 3), out.data_ptr(),
-        _strides_array((b, h), (out.stride(0), hd), 2), _HALF_CODE[q.dtype], b, h, hkv, hd, pages, page_size, ptr,
-        stride, width, lens, most, float(scale), *plan, ws.data_ptr() if size else None, size,
+        index, "paged_attn", "tk_paged_attn", q.data_ptr(), _strides_array(qs, qst, 2), k_pages.data_ptr(),
+        _strides_array(ks, kst, 3), v_pages.data_ptr(), _strides_array(ks, vst, 3), out.data_ptr(),
+        _strides_array((b, h), (out_row, hd), 2), _HALF_CODE[q.dtype], b, h, hkv, hd, pages, page_size, ptr, stride,
+        width, lens, most, float(scale), *plan, ws.data_ptr() if size else None, size,
     )
     return out
 
@@ -654,24 +657,25 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
     16 to 1024.  Sequence b has lengths[b] tokens, these included (``cache_reserve`` comes
     first); token j is row ``j % page_size`` of page ``table[b, j // page_size]``.  Row i of
     the ``new[b]`` (int32 ``[B]``; default and at most n) goes to position
-    ``lengths[b] - new[b] + i``.  Positions that have no page are left out.
+    ``lengths[b] - new[b] + i``.  Positions that have no page are left out.  A page that is
+    written belongs to one row of the table alone, as ``cache_reserve`` and ``cache_fork`` leave it.
     """
     what = "cache_append"
-    index = _check_half(what, "k v k_pages v_pages", k, v, k_pages, v_pages)
-    if k.dim() != 4 or k.shape != v.shape or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
-            k.shape[2] != k_pages.shape[1] or k.shape[3] != k_pages.shape[3]:
+    index, (kst, vst, kpst, vpst) = _check_half(what, "k v k_pages v_pages", k, v, k_pages, v_pages)
+    ks, ps = k.shape, k_pages.shape
+    if len(ks) != 4 or ks != v.shape or len(ps) != 4 or ps != v_pages.shape or ks[2] != ps[1] or ks[3] != ps[3]:
         raise ValueError(f"{what}: k, v [B, n, Hkv, hd] and pages [pages, Hkv, page_size, hd] expected, got "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    b, n, hkv, hd = k.shape
-    pages, _, page_size, _ = k_pages.shape
+                         f"{tuple(ks)}, {tuple(v.shape)}, {tuple(ps)}, {tuple(v_pages.shape)}")
+    b, n, hkv, hd = ks
+    pages, _, page_size, _ = ps
     ptr, stride, width, rows = _check_table(what, table, index)
     if rows != b:
         raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
     _launch_on(
-        index, "cache_append", "tk_cache_append", k.data_ptr(), _strides_of(k, 3), v.data_ptr(), _strides_of(v, 3),
-        k_pages.data_ptr(), _strides_of(k_pages, 3), v_pages.data_ptr(), _strides_of(v_pages, 3), b, n, hkv, hd, pages,
-        page_size, ptr, stride, width, _check_int32(what, "lengths", lengths, index, b),
-        None if new is None else _check_int32(what, "new", new, index, b),
+        index, "cache_append", "tk_cache_append", k.data_ptr(), _strides_array(ks, kst, 3), v.data_ptr(),
+        _strides_array(ks, vst, 3), k_pages.data_ptr(), _strides_array(ps, kpst, 3), v_pages.data_ptr(),
+        _strides_array(ps, vpst, 3), b, n, hkv, hd, pages, page_size, ptr, stride, width,
+        _check_int32(what, "lengths", lengths, index, b), None if new is None else _check_int32(what, "new", new, index, b),
     )
 
 
@@ -700,7 +704,8 @@ def cache_fork(k_pages, v_pages, table, lengths, refs, parents, children):
 
     Whole pages are shared (their refs grow by one); the rows of a page that is only begun
     are copied, in every layer, into a free page, so that both go on writing their own.
-    k_pages and v_pages are ``[layers, pages, Hkv, page_size, hd]`` (or one layer's).  A
+    k_pages and v_pages are ``[layers, pages, Hkv, page_size, hd]`` (or, of a cache of one
+    layer, without the first dimension).  A
     parent may have several children; a child must be an empty row, named once.  Parents
     count as they were before the call.  Returns the status as ``cache_reserve`` does: 0,
     or nothing has changed and it is the number of missing pages, or -1 for a row that is
