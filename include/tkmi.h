@@ -491,8 +491,8 @@ int tk_window_attn(const void *q, const int64_t *q_strides, const void *k,
  * table entry is no page of the cache are not seen; a sequence that sees nothing gets 0.
  * max_length: the longest length to be expected; it only sizes the split of the keys over
  * workgroups, longer sequences are attended whole.  batch_invariant: a sequence's bits do
- * not depend on the rest of the batch or on max_length, which then counts (in the workspace's
- * size too) as at least table_width * page_size.  workspace: tk_paged_attn_workspace bytes, 16-byte
+ * not depend on the rest of the batch, table_width or max_length, which then counts (in the
+ * workspace's size too) as at least table_width * page_size.  workspace: tk_paged_attn_workspace bytes, 16-byte
  * aligned, this call's own until its launches have run (0 bytes: may be NULL).
  */
 int64_t tk_paged_attn_workspace(int64_t batch, int64_t heads, int64_t kv_heads,

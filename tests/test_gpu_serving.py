@@ -290,11 +290,16 @@ def test_paged_long_sequence_splits_and_joins():
     _check_paged(q, k, v, table, lens)
     _check_paged(q, k, v, table, lens, max_length=9000)
     whole = _check_paged(q, k, v, table, lens, batch_invariant=True)
+    kd, vd = k.to(DEV), v.to(DEV)
     for n in range(4):
-        for most in (40000, 100):
-            one = ops.paged_attention(q[n:n + 1].to(DEV), k.to(DEV), v.to(DEV), table[n:n + 1].to(DEV),
-                                      lens[n:n + 1].to(DEV), 1.5 / 8, batch_invariant=True, max_length=most)
-            assert torch.equal(one[0], whole[n])
+        # alone, under other bounds, in a table of its own pages only and in a wider one
+        for width in (table.shape[1], max(-(-lengths[n] // 64), 1), 2 * table.shape[1] + 7):
+            own = torch.full((1, width), -1, dtype=torch.int32)
+            own[:, :min(width, table.shape[1])] = table[n:n + 1, :width]
+            for most in (40000, 100):
+                one = ops.paged_attention(q[n:n + 1].to(DEV), kd, vd, own.to(DEV), lens[n:n + 1].to(DEV), 1.5 / 8,
+                                          batch_invariant=True, max_length=most)
+                assert torch.equal(one[0], whole[n])
 
 
 @pytest.mark.parametrize("b,hkv,longest", [(130, 1, 9000), (70, 2, 9100), (1030, 1, 300), (300, 1, 8300)])
@@ -574,6 +579,32 @@ def test_generation_with_a_cache_matches_whole_sequences(window, sinks):
         # both paths round to fp16 at the same places; a last-bit difference in one (2^-11 of values of
         # a few units) passes through two layers of width 128
         assert float((got - x[starts[b]:]).abs().max()) < 2e-2
+
+
+def test_empty_calls():
+    """No sequences, no heads, no tokens, no pages, no columns."""
+    def half(*shape):
+        return torch.zeros(*shape, dtype=F16, device=DEV)
+
+    def ints(*shape):
+        return torch.zeros(*shape, dtype=torch.int32, device=DEV)
+
+    assert ops.window_attention(half(0, 2, 4, 64), half(0, 1, 4, 64), half(0, 1, 4, 64), 0.1, 4).shape == (0, 4, 128)
+    assert ops.window_attention(half(2, 0, 4, 64), half(2, 0, 4, 64), half(2, 0, 4, 64), 0.1, 4).shape == (2, 4, 0)
+    assert ops.window_attention(half(2, 2, 0, 64), half(2, 1, 4, 64), half(2, 1, 4, 64), 0.1, 4).shape == (2, 0, 128)
+    assert ops.window_attention(half(2, 2, 4, 0), half(2, 1, 4, 0), half(2, 1, 4, 0), 0.1, 4).shape == (2, 4, 0)
+    page = half(3, 1, 16, 64)
+    assert ops.paged_attention(half(0, 2, 64), page, page, ints(0, 4), ints(0), 0.1).shape == (0, 128)
+    assert ops.paged_attention(half(2, 0, 64), half(3, 0, 16, 64), half(3, 0, 16, 64), ints(2, 4), ints(2), 0.1).shape == (2, 0)
+    for pages, width in ((page, 0), (half(0, 1, 16, 64), 4)):  # no entries; no pages: nothing is seen
+        out = ops.paged_attention(half(2, 2, 64) + 1, pages, pages, ints(2, width), ints(2) + 30, 0.1)
+        assert out.shape == (2, 128) and not bool(out.any())
+    ops.cache_append(half(2, 0, 1, 64), half(2, 0, 1, 64), page, page, ints(2, 4), ints(2))
+    ops.cache_append(half(0, 3, 1, 64), half(0, 3, 1, 64), page, page, ints(0, 4), ints(0))
+    assert int(ops.cache_reserve(ints(0, 4), ints(0), ints(5), ints(0), 16)) == 0
+    assert int(ops.cache_compact(page, page, ints(0, 4), ints(0), ints(3))) == 0
+    ops.cache_free(ints(0, 4), ints(0), ints(5), ints(2), 16)
+    assert not bool(page.any())
 
 
 def test_streams_and_two_graphs():

@@ -139,3 +139,21 @@ def test_wrappers_refuse_on_the_cpu():
         ops.cache_compact(half, half, table, vec, vec)
     with pytest.raises(TypeError, match="int32"):
         ops.cache_reserve(table.long(), vec, vec, vec, 16)
+
+
+def test_serving_kernels_use_no_scratch():
+    """A spilled accumulator costs several times a kernel's time and no result shows it."""
+    import json
+
+    from tkmi import build as tkbuild
+
+    if not tkbuild.RESOURCE_PATH.exists():
+        pytest.skip("library not built")
+    usage = json.loads(tkbuild.RESOURCE_PATH.read_text())
+    # types x head-dim tiles x (one or a few workgroups per sequence; masked or not), the joins, the cache's
+    expected = {"paged_attn_kernel": 16, "window_attn_kernel": 16, "window_split_kernel": 16, "split_join_kernel": 4,
+                "cache_": 7}
+    for name, least in expected.items():
+        found = {k: v["scratch"] for k, v in usage.items() if name in k}
+        assert len(found) >= least, (name, len(found))
+        assert not any(found.values()), found

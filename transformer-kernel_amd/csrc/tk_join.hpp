@@ -42,8 +42,8 @@ struct JoinPart {
 // GROUPED: a workgroup joins 16 columns of a row, with 64 groups of 4 lanes; else a wave joins a row, with
 // groups of 16, 32 or 64 lanes.  Group i takes splits i, i + groups, ..., and the groups are merged as one
 // tree, so the sums have one order whatever the batch.  A chain of load latencies (the plan, the results),
-// so nothing waits for the maximum of all splits: 256 splits of 16 rows of 128 take 4.3 us, 2 of 1024 rows
-// 3.5.
+// so nothing waits for the maximum of all splits: 256 splits of 16 rows of 128 take 4.0 us, 2 of 1024 rows
+// 4.8 (the same work behind a first pass for the maximum, and summed group by group, 6.6).
 template <typename T, bool GROUPED>
 __global__ __launch_bounds__(kJoinWaves * 64) void split_join_kernel(JoinArgs p) {
   __shared__ JoinPart lds[GROUPED ? kJoinWaves : 1][4];
@@ -90,8 +90,10 @@ __global__ __launch_bounds__(kJoinWaves * 64) void split_join_kernel(JoinArgs p)
 }
 
 template <typename T>
-int launch_join(const char* fn, const JoinArgs& p, hipStream_t st) {
-  const bool grouped = p.splits > 16;
+int launch_join(const char* fn, const JoinArgs& p, bool one_order, hipStream_t st) {
+  // Few splits: a wave per row.  one_order: the tree of the groups, in which splits that a longer table adds
+  // (empty ones) change no bit.
+  const bool grouped = one_order || p.splits > 16;
   const int64_t grid = grouped ? p.rows * ((p.hd + 15) / 16) : (p.rows + kJoinWaves - 1) / kJoinWaves;
   TK_REQUIRE(grid < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
   const dim3 g((unsigned)grid), blk(kJoinWaves * 64);

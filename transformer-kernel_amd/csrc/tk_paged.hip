@@ -16,7 +16,9 @@
 //     lie (slot 8g + 4t + r), so P needs no move; lane l loads the CW = DT/16 neighbouring
 //     columns of V's rows 16t + 4g + r and one v_perm per pair of keys makes each operand.
 // K's registers are refilled when S is done and V's when O is, so a wave always has about a
-// step's bytes in flight.
+// step's bytes in flight.  Measured: 64 sequences of 16384 tokens, 4 key heads of 128, 6.1 TB/s; 200 of
+// about 1000 visible ones, 16 heads of 64, 5.5; 64 of 100 to 4096, 4 heads of 128 bf16, 4.6 (61 us); one
+// of 100000, 2 heads of 128, 5.1 (20 us) and 4 us for the join.  Fixed cost of a launch: 4.2 us.
 //
 // Where the sequences and key heads alone would leave CUs idle, every sequence's keys are split
 // over workgroups (paged_share), and a second launch joins their results (tk_join.hpp).
@@ -453,9 +455,11 @@ PagedPlan paged_plan(int64_t batch, int64_t per_seq, int64_t max_length, int64_t
     return {batch * (n > 1 ? n : 1), per, false, false};
   }
   const int64_t most = (tiles + kPagedLeast - 1) / kPagedLeast;  // shares of the longest sequence
-  // From half the CUs on, a split of every sequence gains less than the launch that joins it takes: 186 sequences of 676 to 917
-  // tokens, one key head of 64, in whole ones 10.7 us, split 16.8; 17 sequences of 4000, 8 key heads of 128
-  // 57 and 70.  (Below: 2 sequences of 2000 tokens, 2 key heads of 128, 10 us split, 17 whole.)
+  // From half the CUs on, a split of every sequence gains less than the launch that joins it takes: 186
+  // sequences of 676 to 917 tokens, one key head of 64, in whole ones 10.7 us, split 16.8; 17 sequences of
+  // 4000, 8 key heads of 128 57 and 70.  (Below: 2 sequences of 2000 tokens, 2 key heads of 128, 10 us split,
+  // 17 whole.)  Only where a sequence may be long enough to outlast all others are such ones cut: 199
+  // of 100 tokens and one of 60000, one key head of 128, take 25.6 us, whole 524.
   const int64_t whole = kPagedBlocks / 2 / per_seq;  // sequences
   if (batch >= whole) {
     if (tiles < kPagedLong || batch > kShareRows) return {batch, 0, false, false};
@@ -493,7 +497,7 @@ int launch_paged(const PagedArgs& p, int64_t grid, hipStream_t st) {
   j.plan = p.plan;
   j.splits = p.workers / p.batch;
   j.rows = (int64_t)p.batch * p.heads;
-  return launch_join<T>("tk_paged_attn", j, st);
+  return launch_join<T>("tk_paged_attn", j, p.fixed > 0, st);
 }
 
 }  // namespace

@@ -536,7 +536,7 @@ int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   j.hd = p.hd;
   j.splits = p.splits;
   j.rows = (int64_t)p.batch * p.heads * p.q_len;
-  return launch_join<T>(fn, j, st);
+  return launch_join<T>(fn, j, false, st);
 }
 
 template <typename T>

@@ -615,7 +615,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
     cache are not seen; a sequence that sees nothing gets zeros.  ``max_length`` (default:
     the table's) says how long sequences are expected to be: it sizes the split of the keys
     over workgroups and changes no result beyond rounding.  ``batch_invariant``: a
-    sequence's bits do not depend on the batch or ``max_length``.
+    sequence's bits do not depend on the batch, the table's width or ``max_length``.
     """
     what = "paged_attention"
     index, (qst, kst, vst) = _check_half(what, "q k_pages v_pages", q, k_pages, v_pages)
