@@ -455,8 +455,8 @@ int tk_forward(const tk_model *model, const void *x, void *out, int64_t batch, i
  * q [batch, heads, q_len, head_dim], k and v [batch, kv_heads, k_len, head_dim], out as q:
  * element strides {b, h, s} in *_strides[3].  scale > 0.  What K and V hold at keys that
  * are not valid has no effect; at valid ones it must be finite.
- * Launches with few query rows split their keys over workgroups and waves; batch_invariant:
- * not so, a sequence's bits do not depend on the rest of the batch.  workspace:
+ * Launches with few query rows split their keys over workgroups; batch_invariant: not so, a
+ * sequence's bits do not depend on the rest of the batch.  workspace:
  * tk_window_attn_workspace bytes, 16-byte aligned, this call's own until its launches have
  * run (0 bytes: may be NULL).
  */

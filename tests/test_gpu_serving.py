@@ -167,6 +167,42 @@ def test_window_few_rows_and_many_keys(hd):
         _check_window(q, k.masked_fill(bad, float("nan")), v.masked_fill(bad, float("inf")), window, sinks, valid)
 
 
+# fewer than 32 rows a head, groups whose rows end inside, at and past a block of 32; 32 to 65 rows of many heads
+@pytest.mark.parametrize("b,h,hkv,sq", [(1, 4, 1, 8), (2, 10, 2, 7), (3, 6, 2, 16), (2, 14, 2, 31), (1, 66, 1, 1),
+                                        (40, 8, 8, 3), (40, 8, 2, 32), (24, 12, 4, 33), (33, 8, 4, 64), (33, 8, 4, 65)])
+@pytest.mark.parametrize("hd", [24, 64, 104, 256])
+def test_window_short_queries_of_groups(b, h, hkv, sq, hd):
+    sk = sq + 170
+    q, k, v = _window_inputs(b, h, hkv, sq, sk, hd, F16 if sq % 2 else BF16, seed=sq + h)
+    q = q.transpose(1, 2).contiguous().transpose(1, 2)  # heads beside each other, tokens apart
+    _check_window(q, k, v, 75, 3)
+    valid = torch.rand(b, sk, generator=torch.Generator().manual_seed(sq)) > 0.3
+    valid[0, :sk - sq] = False  # rows that see none, some, all of the new keys
+    valid[-1] = False
+    bad = ~valid[:, None, :, None].expand_as(k)
+    out = _check_window(q, k.masked_fill(bad, float("nan")), v.masked_fill(bad, float("inf")), 75, 3, valid)
+    assert not out[:, -1].any()
+
+
+def test_window_short_queries_split_over_workgroups():
+    """A group's rows in two blocks, whose keys go to several workgroups: joined per head and row."""
+    for dtype, hd in [(F16, 64), (BF16, 128), (F16, 200)]:
+        q, k, v = _window_inputs(2, 10, 2, 7, 6000, hd, dtype, seed=hd)
+        _check_window(q, k, v, 5000, 9)
+        valid = torch.ones(2, 6000, dtype=torch.bool)
+        valid[0, 1500:5996] = False
+        _check_window(q, k, v, 5000, 9, valid)
+
+
+def test_window_short_queries_leave_what_lies_around_them():
+    q, k, v = (t.to(DEV) for t in _window_inputs(2, 10, 2, 7, 300, 64, F16))
+    buf = torch.full((2, 9, 10 * 64 + 8), 7.0, dtype=F16, device=DEV)
+    ops.window_attention(q, k, v, 0.1, 100, sinks=2, out=buf[:, 1:-1, 4:-4])
+    assert torch.equal(buf[:, 1:-1, 4:-4], ops.window_attention(q, k, v, 0.1, 100, sinks=2))
+    buf[:, 1:-1, 4:-4] = 7.0
+    assert bool((buf == 7.0).all())
+
+
 # ------------------------------------------------------------------- paged --
 
 

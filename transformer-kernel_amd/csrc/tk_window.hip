@@ -34,7 +34,8 @@ struct WindowArgs {
   int64_t qs[3], ks[3], vs[3], os[3];  // elements, {b, h, s}
   int batch, heads, group, q_len, k_len, hd, window, sinks;
   int n_qt;
-  int splits, per_split;  // window_split_kernel: key tiles of a workgroup
+  int unit;               // window_split_kernel: heads whose rows, one head's after another's, make one list
+  int splits, per_split;  //   and key tiles of a workgroup
   float* part;            // its results where splits > 1 (tk_join.hpp)
   float* stats;
   float scale_log2;
@@ -247,13 +248,13 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
 }
 
 // The same rows' keys dealt to the waves of a workgroup (and to several workgroups): for launches with too
-// few query rows to fill the chip, whose workgroups of the kernel above would walk their tiles as one
-// serial chain each.  32 rows of one head per workgroup; wave w takes every NW-th of its tiles of kSplitKeys
-// keys, into K and V slots of its own, so the loop has no barrier: the next K is copied when the current
-// one's products are done, the next V after P.V.  At the end the waves' (max, sum, O) are merged in wave
-// order.  Tiles of 32 keys leave room for two to six workgroups per CU: 16 heads of 64, 619 rows, window 126
-// 9.0 us, with tiles of 64 11.7.  (Two waves of rows per tile, tiles ahead in a second slot: 14.0, and 31 us
-// instead of 38 where a window of 2048 keys makes the chains long.)
+// few query rows to fill the chip, whose workgroups of the kernel above would walk their tiles as one serial
+// chain each.  32 rows of one head per workgroup, or of a group's heads one after the other; wave w takes
+// every NW-th of its tiles of kSplitKeys keys, into K and V slots of its own, so the loop has no barrier: the
+// next K is copied when the current one's products are done, the next V after P.V.  At the end the waves'
+// (max, sum, O) are merged in wave order.  Tiles of 32 keys leave room for two to six workgroups per CU: 16
+// heads of 64, 619 rows, window 126 9.0 us, with tiles of 64 11.7.  (Two waves of rows per tile, tiles ahead
+// in a second slot: 14.0, and 31 us instead of 38 where a window of 2048 keys makes the chains long.)
 constexpr int kSplitKeys = 32;
 template <typename T, int DT, int NW, bool KMASK>
 __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
@@ -278,16 +279,17 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
   // as in window_body, an XCD takes neighbouring blocks
-  const int total = p.n_qt * p.batch * p.heads * p.splits, per = (total + 7) / 8;
+  const int units = p.heads / p.unit, total = p.n_qt * p.batch * units * p.splits, per = (total + 7) / 8;
   int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= total) return;
   const int split = id % p.splits;
   id /= p.splits;
-  const int qt = id % p.n_qt, bh = id / p.n_qt;
-  const int b = bh / p.heads, h = bh % p.heads, kvh = h / p.group;
+  const int qt = id % p.n_qt, bu = id / p.n_qt;
+  const int b = bu / units, h0 = bu % units * p.unit, kvh = h0 / p.group;
 
-  const int q0 = qt * 32, shift = p.k_len - p.q_len;
-  const int row = q0 + (lane & 31), pos = shift + row;
+  // several heads make a list only where each has fewer than 32 rows: the block may hold any of them
+  const int q0 = p.unit > 1 ? 0 : qt * 32, shift = p.k_len - p.q_len;
+  const int in_list = min(qt * 32 + (lane & 31), p.unit * p.q_len - 1), pos = shift + in_list % p.q_len;
   const int w_lo = shift + q0, w_hi = min(w_lo + 31, p.k_len - 1);
   const TileList<BN> tiles(p, w_lo, w_hi);
   const int t_end = min(tiles.n, (split + 1) * p.per_split);
@@ -313,7 +315,8 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
 
   x8 qf[KSTEPS];
   {
-    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + (int64_t)min(row, p.q_len - 1) * p.qs[2];
+    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + (h0 + in_list / p.q_len) * p.qs[1] +
+                  (in_list % p.q_len) * p.qs[2];
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) {
       const int d = 16 * kk + 8 * g;
@@ -402,9 +405,10 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
     asm volatile("" ::: "memory");
     if (KMASK && bits != ~0ull >> (64 - BN)) {
       // whatever lies in rows that are not valid times a weight of 0 must be 0
+      const uint32_t mine = (uint32_t)bits >> (lane / CPR);
 #pragma unroll
       for (int c = 0; c < COPIES; ++c)
-        if (!((bits >> (c * RPC + lane / CPR)) & 1)) *reinterpret_cast<u32x4*>(vs_ + c * 1024 + lane * 16) = u32x4{};
+        if (!((mine >> (c * RPC)) & 1)) *reinterpret_cast<u32x4*>(vs_ + c * 1024 + lane * 16) = u32x4{};
       wait_lds_reads();
       asm volatile("" ::: "memory");
     }
@@ -449,10 +453,14 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
     f[w] = __builtin_amdgcn_exp2f(f[w] - m_ref);
     l_all = fmaf(f[w], row_l[w][lane & 31], l_all);
   }
-  if (row >= p.q_len) return;
+  int listed = lane & 31;
+  asm volatile("" : "+v"(listed));  // head and row found anew: they need no registers in the loop
+  listed += qt * 32;
+  if (listed >= p.unit * p.q_len) return;
+  const int h = h0 + listed / p.q_len, row = listed % p.q_len;
   const float inv = l_all == 0.f ? 0.f : 1.0f / l_all;
-  T* orow = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + (int64_t)row * p.os[2];
-  const int64_t part = ((int64_t)bh * p.q_len + row) * p.splits + split;
+  T* orow = reinterpret_cast<T*>(p.o) + b * p.os[0] + h * p.os[1] + row * p.os[2];
+  const int64_t part = (((int64_t)b * p.heads + h) * p.q_len + row) * p.splits + split;
   if (p.splits > 1 && wave == 0 && g == 0) {
     p.stats[2 * part] = m_all;
     p.stats[2 * part + 1] = l_all;
@@ -485,19 +493,31 @@ __global__ __launch_bounds__(NW * 64, DT <= 128 ? 2 : 1) void window_attn_kernel
 
 constexpr int kWindowWaves = 4;
 
-// Which kernel, and over how many workgroups window_split_kernel deals a block of 32 rows' keys.
+// Which kernel; for window_split_kernel the heads whose rows make one list, its blocks of 32 rows, and over how
+// many workgroups a block's keys are dealt.
 struct WindowPlan {
   bool split;
+  int64_t unit, blocks;
   int64_t splits, per_split;
 };
-WindowPlan window_plan(int64_t bh, int64_t q_len, int64_t k_len, int64_t window, int64_t sinks, int64_t hd,
-                       bool batch_invariant) {
-  // Workgroups of 128 rows fill the chip from one per CU on (two at head_dim 256, one wave per SIMD).
-  if (batch_invariant || bh * ((q_len + 127) / 128) > (hd > 128 ? 512 : 256)) return {false, 1, 0};
+WindowPlan window_plan(int64_t bh, int64_t group, int64_t q_len, int64_t k_len, int64_t window, int64_t sinks,
+                       int64_t hd, bool batch_invariant) {
+  // Workgroups of 128 rows fill the chip from one per CU on (two at head_dim 256, one wave per SIMD).  Up to 64
+  // rows a head (32 above head_dim 64) half of their waves or more have none, however many heads there are: 64 x
+  // 16 heads in groups of 4, window 2048, us by rows: head_dim 32 65 with 128-row workgroups, 50 in blocks of 32 at
+  // 64 rows, 69 and 71 at 80; head_dim 64 92 and 85 at 64, 102 and 117 at 80; head_dim 128 162 and 99 at 32, 162
+  // and 167 at 48.
+  const int64_t wide = bh * ((q_len + 127) / 128);
+  const bool few = q_len <= (hd > 64 ? 32 : 64);
+  if (!few && (batch_invariant || wide > (hd > 128 ? 512 : 256))) return {false, 1, wide, 1, 0};
+  // Fewer than 32 rows a head: those of a group, which read the same keys, fill the blocks (9 x 32 heads in groups
+  // of 4, 8 rows, 3487 keys, head_dim 80: 24 us, a workgroup per head 98).
+  const int64_t unit = q_len < 32 && group < (1 << 26) ? group : 1, blocks = bh / unit * ((unit * q_len + 31) / 32);
   int64_t keys = window + 31 + sinks;
   if (keys > k_len) keys = k_len;
   // the sinks and the windows may begin and end inside tiles
-  const int64_t tiles = (keys + kSplitKeys - 1) / kSplitKeys + 2, blocks = bh * ((q_len + 31) / 32);
+  const int64_t tiles = (keys + kSplitKeys - 1) / kSplitKeys + 2;
+  if (batch_invariant) return {true, unit, blocks, 1, tiles};
   // A block's keys go to several workgroups only up to one workgroup per CU, in shares of three tiles a wave or
   // more: past that the launch that joins them costs more (10 x 2 heads of 128, 735 rows: whole 20 us, in two
   // 38; 3 heads of 64, 923 rows, window 2920: 18 us in eight shares, 34 whole).
@@ -505,16 +525,16 @@ WindowPlan window_plan(int64_t bh, int64_t q_len, int64_t k_len, int64_t window,
   int64_t per = (tiles + want - 1) / want;
   per = (per + kWindowWaves - 1) / kWindowWaves * kWindowWaves;
   if (per < 3 * kWindowWaves) per = 3 * kWindowWaves;
-  return {true, (tiles + per - 1) / per, per};
+  return {true, unit, blocks, (tiles + per - 1) / per, per};
 }
 
 template <typename T, int DT, int BN>
 int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   constexpr int NW = kWindowWaves;
   const char* fn = "tk_window_attn";
-  const int rows = plan.split ? 32 : 32 * NW;
-  p.n_qt = (p.q_len + rows - 1) / rows;
-  const int64_t total = (int64_t)p.n_qt * p.batch * p.heads * plan.splits;
+  p.unit = (int)plan.unit;
+  p.n_qt = (int)(plan.blocks / ((int64_t)p.batch * (p.heads / p.unit)));
+  const int64_t total = plan.blocks * plan.splits;
   TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
   const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
   if (!plan.split) {
@@ -586,8 +606,8 @@ extern "C" int64_t tk_window_attn_workspace(int64_t batch, int64_t heads, int64_
                                     sinks);
   if (rc != TK_OK) return rc;
   if (batch == 0 || heads == 0 || q_len == 0) return 0;
-  return window_workspace(window_plan(batch * heads, q_len, k_len, at_most(window, k_len), at_most(sinks, k_len),
-                                      head_dim, batch_invariant != 0),
+  return window_workspace(window_plan(batch * heads, heads / kv_heads, q_len, k_len, at_most(window, k_len),
+                                      at_most(sinks, k_len), head_dim, batch_invariant != 0),
                           batch * heads * q_len, head_dim);
 }
 
@@ -632,7 +652,8 @@ extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const voi
   p.window = (int)at_most(window, k_len);
   p.sinks = (int)at_most(sinks, k_len);
   p.scale_log2 = scale * 1.4426950408889634f;
-  const WindowPlan plan = window_plan(batch * heads, q_len, k_len, p.window, p.sinks, head_dim, batch_invariant != 0);
+  const WindowPlan plan =
+      window_plan(batch * heads, p.group, q_len, k_len, p.window, p.sinks, head_dim, batch_invariant != 0);
   const int64_t rows = batch * heads * q_len, need = window_workspace(plan, rows, head_dim);
   TK_REQUIRE(need == 0 || (workspace && al(workspace, 16) && workspace_bytes >= need), TK_ERR_ARG,
              "%s: workspace of %lld bytes, 16-byte aligned, needed", fn, (long long)need);
