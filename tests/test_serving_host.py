@@ -120,6 +120,19 @@ def test_cache_calls_refuse():
     assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (6 + 16)
 
 
+def test_launches_of_too_many_workgroups_are_refused():
+    """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256."""
+    lib = _lib.load()
+    state = (16, 4, 4, 1 << 18, 16, 16, 8, 16)
+    assert _window(b=1 << 20, h=32, hkv=32) == -2
+    assert _window(b=1 << 20, h=32, hkv=32, sq=300, sk=300) == -2
+    assert _paged(b=1 << 23) == -2
+    assert lib.tk_cache_append(16, S3, 16, S3, 16, S3, 16, S3, 1 << 14, 1 << 15, 1, 64, 4, 16, 16, 4, 4, 16, None,
+                               None) == -2
+    assert lib.tk_cache_fork(16, S4, 16, S4, 2, 2, 64, *state, 16, 16, 1 << 22, 16, 16, 1 << 40, None) == -2
+    assert lib.tk_cache_free(*state, 16, 1 << 24, None) == -1
+
+
 def test_wrappers_refuse_on_the_cpu():
     half = torch.zeros(1, 2, 4, 64, dtype=torch.float16)
     table, vec = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)

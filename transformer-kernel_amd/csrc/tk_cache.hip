@@ -554,7 +554,7 @@ extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const vo
   p.page_shift = __builtin_ctzll((unsigned long long)page_size);
   p.table_width = (int)table_width;
   const int64_t items = n * kv_heads * p.vecs, blocks = (items + 255) / 256;
-  TK_REQUIRE(items < (1ll << 31) - 256 && blocks * batch < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  TK_REQUIRE(items < (1ll << 31) - 256 && blocks * batch <= kMaxGroups, TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
   p.blocks = (int)blocks;
   hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)(blocks * batch)), dim3(256), 0, as_stream(stream), p);
   return check_launch(fn);
@@ -592,7 +592,7 @@ extern "C" int tk_cache_fork(void* k_pages, const int64_t* k_strides, void* v_pa
   TK_REQUIRE(rows <= kForkRows, TK_ERR_UNSUPPORTED, "%s: a table of more than %d rows", fn, kForkRows);
   if ((rc = check_workspace(fn, workspace, workspace_bytes, 4 * (2 * n + pages))) != TK_OK) return rc;
   const int64_t grid = n * (1 + (int64_t)p.layers * p.kv_heads);
-  TK_REQUIRE(grid < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many children", fn);
+  TK_REQUIRE(grid <= kMaxGroups, TK_ERR_UNSUPPORTED, "%s: too many children", fn);
   p.first = parents;
   p.second = children;
   p.n = (int)n;
@@ -611,7 +611,7 @@ extern "C" int tk_cache_free(int32_t* table, int64_t table_stride, int64_t table
   CacheArgs p{};
   const int rc = fill_cache(fn, p, table, table_stride, table_width, rows, lengths, refs, pages, page_size);
   if (rc != TK_OK) return rc;
-  TK_REQUIRE(n >= 0 && n < (1ll << 31) && (n == 0 || list), TK_ERR_ARG, "%s: bad list of rows", fn);
+  TK_REQUIRE(n >= 0 && n <= kMaxGroups && (n == 0 || list), TK_ERR_ARG, "%s: bad list of rows", fn);
   if (n == 0) return TK_OK;
   p.first = list;
   p.n = (int)n;

@@ -11,6 +11,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// Workgroups of 256 threads in a launch, which holds fewer than 2^32 threads.
+constexpr int64_t kMaxGroups = (1 << 24) - 8;
+
 template <typename T>
 struct Elem;
 

@@ -95,7 +95,7 @@ int launch_join(const char* fn, const JoinArgs& p, bool one_order, hipStream_t s
   // (empty ones) change no bit.
   const bool grouped = one_order || p.splits > 16;
   const int64_t grid = grouped ? p.rows * ((p.hd + 15) / 16) : (p.rows + kJoinWaves - 1) / kJoinWaves;
-  TK_REQUIRE(grid < (1ll << 31), TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  TK_REQUIRE(grid <= kMaxGroups, TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
   const dim3 g((unsigned)grid), blk(kJoinWaves * 64);
   if (grouped) hipLaunchKernelGGL((split_join_kernel<T, true>), g, blk, 0, st, p);
   else hipLaunchKernelGGL((split_join_kernel<T, false>), g, blk, 0, st, p);

@@ -535,7 +535,7 @@ int launch_window(WindowArgs p, const WindowPlan& plan, hipStream_t st) {
   p.unit = (int)plan.unit;
   p.n_qt = (int)(plan.blocks / ((int64_t)p.batch * (p.heads / p.unit)));
   const int64_t total = plan.blocks * plan.splits;
-  TK_REQUIRE(total < (1ll << 31) - 8, TK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  TK_REQUIRE(total <= kMaxGroups, TK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
   const dim3 g((unsigned)((total + 7) / 8 * 8)), blk(NW * 64);
   if (!plan.split) {
     if (p.kv) hipLaunchKernelGGL((window_attn_kernel<T, DT, BN, NW, true>), g, blk, 0, st, p);
