@@ -167,9 +167,10 @@ def test_window_few_rows_and_many_keys(hd):
         _check_window(q, k.masked_fill(bad, float("nan")), v.masked_fill(bad, float("inf")), window, sinks, valid)
 
 
-# fewer than 32 rows a head, groups whose rows end inside, at and past a block of 32; 32 to 65 rows of many heads
+# fewer than 32 rows a head, groups whose rows end inside, at and past a block of 32; 32 to 96 rows of many heads
 @pytest.mark.parametrize("b,h,hkv,sq", [(1, 4, 1, 8), (2, 10, 2, 7), (3, 6, 2, 16), (2, 14, 2, 31), (1, 66, 1, 1),
-                                        (40, 8, 8, 3), (40, 8, 2, 32), (24, 12, 4, 33), (33, 8, 4, 64), (33, 8, 4, 65)])
+                                        (40, 8, 8, 3), (40, 8, 2, 32), (24, 12, 4, 33), (33, 8, 4, 64), (33, 8, 4, 65),
+                                        (50, 8, 4, 33), (50, 8, 4, 96)])
 @pytest.mark.parametrize("hd", [24, 64, 104, 256])
 def test_window_short_queries_of_groups(b, h, hkv, sq, hd):
     sk = sq + 170

@@ -174,8 +174,8 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
     }
     lds_barrier();
     if (t + 1 < tiles.n) copy(t + 1, lds0 + ((t + 1) & 1) * 2 * TILE);
-    // nothing of this tile for any of the wave's rows
-    if (k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
+    // nothing of this tile for any of the wave's rows, or no rows (1024 heads of 64, 200 rows: 69.6 -> 63.1 us)
+    if (w_lo >= p.k_len || k0 > w_hi || (k0 + BN - 1 <= w_lo - p.window && k0 >= p.sinks)) continue;
 
     // the products ahead of another wave's exponentials: 588 -> 568 us at head_dim 128
     f32x16 s[NB];
@@ -502,14 +502,14 @@ struct WindowPlan {
 };
 WindowPlan window_plan(int64_t bh, int64_t group, int64_t q_len, int64_t k_len, int64_t window, int64_t sinks,
                        int64_t hd, bool batch_invariant) {
-  // Workgroups of 128 rows fill the chip from one per CU on (two at head_dim 256, one wave per SIMD).  Up to 64
-  // rows a head (32 above head_dim 64) half of their waves or more have none, however many heads there are: 64 x
-  // 16 heads in groups of 4, window 2048, us by rows: head_dim 32 65 with 128-row workgroups, 50 in blocks of 32 at
-  // 64 rows, 69 and 71 at 80; head_dim 64 92 and 85 at 64, 102 and 117 at 80; head_dim 128 162 and 99 at 32, 162
-  // and 167 at 48.
-  const int64_t wide = bh * ((q_len + 127) / 128);
-  const bool few = q_len <= (hd > 64 ? 32 : 64);
-  if (!few && (batch_invariant || wide > (hd > 128 ? 512 : 256))) return {false, 1, wide, 1, 0};
+  // Workgroups of 128 rows fill the chip from one per CU on; two at head_dim 256 (one wave per SIMD), and three to
+  // two CUs where a quarter of their waves has no rows and the tiles are short: head_dim 64 and 64 rows, window 512,
+  // us in blocks of 32 rows and of 128: 272 heads 15.1, 18.7; 384 14.0, 18.6; 512 21.2, 20.0.  Up to 32 rows a head
+  // blocks of 32 win however many heads there are (1024 heads of 128 in groups of 4, window 512: 31, 38; of 256 89,
+  // 119), or come close (320 heads of 128, window 2048: 80, 76).
+  const int64_t wide = bh * ((q_len + 127) / 128), full = hd > 128 ? 512 : hd <= 64 && q_len <= 96 ? 384 : 256;
+  const bool few = q_len <= 32;
+  if (!few && (batch_invariant || wide > full)) return {false, 1, wide, 1, 0};
   // Fewer than 32 rows a head: those of a group, which read the same keys, fill the blocks (9 x 32 heads in groups
   // of 4, 8 rows, 3487 keys, head_dim 80: 24 us, a workgroup per head 98).
   const int64_t unit = q_len < 32 && group < (1 << 26) ? group : 1, blocks = bh / unit * ((unit * q_len + 31) / 32);
