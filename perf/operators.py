@@ -12,7 +12,6 @@ gives further ones of the same ranges.
 
 from __future__ import annotations
 
-import functools
 import math
 import pathlib
 import sys
@@ -269,9 +268,7 @@ def prepare(case, seed):
 # --------------------------------------------------------------------------- #
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
-    """The library's operators, imported at the first call as a program imports them once."""
     package = str(pathlib.Path(__file__).resolve().parents[1] / "transformer-kernel_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
