@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define TKMI_ABI_VERSION 6
+#define TKMI_ABI_VERSION 7
 
 typedef uint16_t tk_half;
 
@@ -515,6 +515,9 @@ int tk_paged_attn(const void *q, const int64_t *q_strides, const void *k_pages,
  * row i < added[b] of k and v [batch, n, kv_heads, head_dim], strides {b, token, head}, goes
  * to position lengths[b] - added[b] + i.  Positions before 0, past the table, or on an entry
  * that is no page of the cache are left out.  Pages of one layer, strides {page, head, row}.
+ * A reservation that was refused has left lengths as they were, so its tokens would be written
+ * over the newest ones of every sequence: tk_cache_append_reserved takes the reservation's status
+ * (device) and writes nothing where it is not 0.
  */
 int tk_cache_append(const void *k, const int64_t *k_strides, const void *v,
                     const int64_t *v_strides, void *k_pages,
@@ -524,6 +527,16 @@ int tk_cache_append(const void *k, const int64_t *k_strides, const void *v,
                     int64_t page_size, const int32_t *table,
                     int64_t table_stride, int64_t table_width,
                     const int32_t *lengths, const int32_t *added, void *stream);
+int tk_cache_append_reserved(const void *k, const int64_t *k_strides,
+                             const void *v, const int64_t *v_strides,
+                             void *k_pages, const int64_t *k_page_strides,
+                             void *v_pages, const int64_t *v_page_strides,
+                             int64_t batch, int64_t n, int64_t kv_heads,
+                             int64_t head_dim, int64_t pages,
+                             int64_t page_size, const int32_t *table,
+                             int64_t table_stride, int64_t table_width,
+                             const int32_t *lengths, const int32_t *added,
+                             const int32_t *status, void *stream);
 
 /*
  * Page bookkeeping, decided on the device.  An operation that cannot be done whole changes

@@ -389,6 +389,23 @@ def test_append_out_of_place_counts():
     assert torch.equal(got_v.cpu().view(torch.int16), v.view(torch.int16))
 
 
+def test_append_of_a_refused_reservation():
+    """The reservation's status, not 0: no byte of the cache changes; 0: as without it."""
+    for status in (0, 1, -1):
+        k, v, table, lens = _cache([40, 1, 33], 2, 64, 16, F16, seed=25)
+        new_k, new_v = seeded(3, 2, 2, 64, dtype=F16, seed=26), seeded(3, 2, 2, 64, dtype=F16, seed=27)
+        new = torch.tensor([2, 1, 1], dtype=torch.int32, device=DEV)
+        got_k, got_v, want_k, want_v = (t.to(DEV) for t in (k, v, k, v))
+        ops.cache_append(new_k.to(DEV), new_v.to(DEV), got_k, got_v, table.to(DEV), lens.to(DEV), new=new,
+                         status=torch.tensor([status], dtype=torch.int32, device=DEV))
+        if status == 0:
+            ops.cache_append(new_k.to(DEV), new_v.to(DEV), want_k, want_v, table.to(DEV), lens.to(DEV), new=new)
+        assert torch.equal(got_k.view(torch.int16), want_k.view(torch.int16))
+        assert torch.equal(got_v.view(torch.int16), want_v.view(torch.int16))
+    with pytest.raises(ValueError, match="status must have 1 entries"):
+        ops.cache_append(new_k.to(DEV), new_v.to(DEV), got_k, got_v, table.to(DEV), lens.to(DEV), status=new)
+
+
 class _State:
     """A cache on the device beside the Book that says what it must hold."""
 
@@ -616,6 +633,50 @@ def test_generation_with_a_cache_matches_whole_sequences(window, sinks):
         # both paths round to fp16 at the same places; a last-bit difference in one (2^-11 of values of
         # a few units) passes through two layers of width 128
         assert float((got - x[starts[b]:]).abs().max()) < 2e-2
+
+
+def test_a_captured_step_that_runs_out_of_pages():
+    """A decode step over forked sequences, captured, replayed while pages are missing: every byte of the cache, the
+    table, lengths and refs stay; once a sequence has ended, the same graph goes on where it was."""
+    layers, heads, hkv, ps, hd, scale = 2, 4, 2, 16, 32, 0.25
+    s = _State(rows=4, width=4, pages=6, layers=layers, hkv=hkv, ps=ps, hd=hd)
+    s.reserve([32, 20, 0, 0]).fork([0, 1], [2, 3])  # whole pages shared, one begun page copied: one page is free
+    one = s.vec([1, 1, 1, 1])
+    rows = [seeded(4, (heads + 2 * hkv), hd, dtype=F16, seed=70 + i).to(DEV) for i in range(layers)]
+    status, outs = s.vec([0]), [torch.zeros(4, heads * hd, dtype=F16, device=DEV) for _ in range(layers)]
+
+    def step():
+        left = ops.cache_reserve(s.table, s.lengths, s.refs, one, ps)
+        for i in range(layers):
+            q, kk, vv = rows[i][:, :heads], rows[i][:, heads:heads + hkv], rows[i][:, heads + hkv:]
+            ops.cache_append(kk[:, None], vv[:, None], s.k[i], s.v[i], s.table, s.lengths, new=one, status=left)
+            outs[i].copy_(ops.paged_attention(q, s.k[i], s.v[i], s.table, s.lengths, scale))
+        status.copy_(left)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for run in (graph.replay, graph.replay, step):  # rows 0 and 2 need a page each
+        run()
+        assert int(status) == s.book.reserve([1, 1, 1, 1]) == 1
+        s.check()
+    s.free([3])  # its copied page is free, the shared one lives on in row 1
+    one[3] = 0
+    for t in range(2):
+        for i in range(layers):
+            rows[i].copy_(seeded(4, (heads + 2 * hkv), hd, dtype=F16, seed=80 + 2 * t + i))
+        graph.replay()
+        assert int(status) == s.book.reserve([1, 1, 1, 0]) == 0
+        for i in range(layers):
+            for b in range(3):
+                page, at = s.book.table[b][(s.book.lengths[b] - 1) // ps], (s.book.lengths[b] - 1) % ps
+                s.want_k[i, page, :, at] = rows[i][b, heads:heads + hkv].cpu()
+                s.want_v[i, page, :, at] = rows[i][b, heads + hkv:].cpu()
+        s.check()
+        for i in range(layers):
+            want, tol = paged_reference(rows[i][:, :heads].cpu(), s.want_k[i], s.want_v[i], s.table.cpu(),
+                                        s.lengths.cpu(), scale)
+            _inside(outs[i], want, tol)
 
 
 def test_empty_calls():

@@ -120,6 +120,20 @@ def test_cache_calls_refuse():
     assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (6 + 16)
 
 
+def test_append_with_a_status_refuses():
+    """As without one, and a status that is not there."""
+    lib = _lib.load()
+
+    def append(hd=64, ps=16, n=1, status=16, lengths=16):
+        return lib.tk_cache_append_reserved(16, S3, 16, S3, 16, S3, 16, S3, 1, n, 1, hd, 4, ps, 16, 4, 4, lengths, None,
+                                            status, None)
+
+    for call, code in [(dict(status=None), -1), (dict(hd=12), -2), (dict(ps=24), -2), (dict(lengths=None), -1),
+                       (dict(n=0), 0)]:
+        assert append(**call) == code, call
+        assert code == 0 or "tk_cache_append_reserved" in lib.tk_last_error_string().decode()
+
+
 def test_launches_of_too_many_workgroups_are_refused():
     """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256."""
     lib = _lib.load()

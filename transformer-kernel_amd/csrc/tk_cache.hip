@@ -35,6 +35,7 @@ struct AppendArgs {
   const int32_t* table;
   const int32_t* lengths;
   const int32_t* added;          // nullable: n of every sequence
+  const int32_t* status;         // nullable: of the call that made room; nothing is written where it is not 0
   int64_t ks[3], vs[3];          // bytes, {b, token, head}
   int64_t kps[3], vps[3];        // bytes, {page, head, row}
   int64_t table_stride;
@@ -47,7 +48,8 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs p) {
   const int x = item % p.vecs, r = item / p.vecs;
   const int h = r % p.kv_heads, i = r / p.kv_heads;
   const int n = p.added ? min(p.added[b], p.n) : p.n;
-  if (i >= n) return;
+  // a refused reservation left lengths as they were: the rows would land on the newest tokens that are there
+  if (i >= n || (p.status && *p.status != 0)) return;
   const int64_t pos = (int64_t)p.lengths[b] - n + i;
   if (pos < 0 || (pos >> p.page_shift) >= p.table_width) return;
   const int page = p.table[b * p.table_stride + (pos >> p.page_shift)];
@@ -517,13 +519,13 @@ extern "C" int64_t tk_cache_workspace(int64_t rows, int64_t pages, int64_t n) {
   return 4 * (2 * n + 2 * pages + 1);
 }
 
-extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                               void* k_pages, const int64_t* k_page_strides, void* v_pages,
-                               const int64_t* v_page_strides, int64_t batch, int64_t n, int64_t kv_heads,
-                               int64_t head_dim, int64_t pages, int64_t page_size, const int32_t* table,
-                               int64_t table_stride, int64_t table_width, const int32_t* lengths,
-                               const int32_t* added, void* stream) {
-  const char* fn = "tk_cache_append";
+namespace {
+
+int append(const char* fn, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+           void* k_pages, const int64_t* k_page_strides, void* v_pages, const int64_t* v_page_strides, int64_t batch,
+           int64_t n, int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, const int32_t* table,
+           int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* added,
+           const int32_t* status, void* stream) {
   int rc = check_table(fn, table, table_stride, table_width, batch, lengths, page_size);
   if (rc != TK_OK) return rc;
   if ((rc = check_head_dim(fn, head_dim)) != TK_OK) return rc;
@@ -542,6 +544,7 @@ extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const vo
   p.table = table;
   p.lengths = lengths;
   p.added = added;
+  p.status = status;
   if ((rc = take_strides(fn, p.ks, k_strides, 3)) != TK_OK || (rc = take_strides(fn, p.vs, v_strides, 3)) != TK_OK ||
       (rc = take_strides(fn, p.kps, k_page_strides, 3)) != TK_OK ||
       (rc = take_strides(fn, p.vps, v_page_strides, 3)) != TK_OK)
@@ -558,6 +561,32 @@ extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const vo
   p.blocks = (int)blocks;
   hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)(blocks * batch)), dim3(256), 0, as_stream(stream), p);
   return check_launch(fn);
+}
+
+}  // namespace
+
+extern "C" int tk_cache_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                               void* k_pages, const int64_t* k_page_strides, void* v_pages,
+                               const int64_t* v_page_strides, int64_t batch, int64_t n, int64_t kv_heads,
+                               int64_t head_dim, int64_t pages, int64_t page_size, const int32_t* table,
+                               int64_t table_stride, int64_t table_width, const int32_t* lengths,
+                               const int32_t* added, void* stream) {
+  return append("tk_cache_append", k, k_strides, v, v_strides, k_pages, k_page_strides, v_pages, v_page_strides, batch,
+                n, kv_heads, head_dim, pages, page_size, table, table_stride, table_width, lengths, added, nullptr,
+                stream);
+}
+
+extern "C" int tk_cache_append_reserved(const void* k, const int64_t* k_strides, const void* v,
+                                        const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides,
+                                        void* v_pages, const int64_t* v_page_strides, int64_t batch, int64_t n,
+                                        int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
+                                        const int32_t* table, int64_t table_stride, int64_t table_width,
+                                        const int32_t* lengths, const int32_t* added, const int32_t* status,
+                                        void* stream) {
+  const char* fn = "tk_cache_append_reserved";
+  TK_REQUIRE(status, TK_ERR_ARG, "%s: null pointer", fn);
+  return append(fn, k, k_strides, v, v_strides, k_pages, k_page_strides, v_pages, v_page_strides, batch, n, kv_heads,
+                head_dim, pages, page_size, table, table_stride, table_width, lengths, added, status, stream);
 }
 
 extern "C" int tk_cache_reserve(int32_t* table, int64_t table_stride, int64_t table_width, int64_t rows,

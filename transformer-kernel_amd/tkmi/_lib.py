@@ -13,7 +13,7 @@ import threading
 from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_void_p
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libtkmi.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 TK_OK, TK_ERR_ARG, TK_ERR_UNSUPPORTED, TK_ERR_HIP = 0, -1, -2, -3
 TK_F32, TK_F16, TK_BF16 = 0, 1, 2
@@ -135,6 +135,11 @@ SIGNATURES = {
     "tk_cache_append": (
         c_int,
         [c_void_p, _STRIDES] * 4 + [c_int64] * 6 + [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    "tk_cache_append_reserved": (
+        c_int,
+        [c_void_p, _STRIDES] * 4 + [c_int64] * 6
+        + [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "tk_cache_reserve": (c_int, _TABLE + [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "tk_cache_fork": (

@@ -649,7 +649,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale: float, window: i
     return out
 
 
-def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
+def cache_append(k, v, k_pages, v_pages, table, lengths, new=None, status=None) -> None:
     """Writes the newest tokens' keys and values into the pages of one layer.
 
     k and v are ``[B, n, Hkv, hd]`` (views of a fused projection's output, for instance);
@@ -659,6 +659,9 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
     the ``new[b]`` (int32 ``[B]``; default and at most n) goes to position
     ``lengths[b] - new[b] + i``.  Positions that have no page are left out.  A page that is
     written belongs to one row of the table alone, as ``cache_reserve`` and ``cache_fork`` leave it.
+    ``status``: what ``cache_reserve`` returned for these tokens; where it is not 0 nothing is written.
+    (A refused reservation leaves lengths as they were, so without it the rows would land on the
+    newest tokens that are there, in pages that other sequences may share.)
     """
     what = "cache_append"
     index, (kst, vst, kpst, vpst) = _check_half(what, "k v k_pages v_pages", k, v, k_pages, v_pages)
@@ -671,11 +674,15 @@ def cache_append(k, v, k_pages, v_pages, table, lengths, new=None) -> None:
     ptr, stride, width, rows = _check_table(what, table, index)
     if rows != b:
         raise ValueError(f"{what}: table must have a row per sequence ({b}), got {rows}")
+    fn, of = "tk_cache_append", ()
+    if status is not None:
+        fn, of = "tk_cache_append_reserved", (_check_int32(what, "status", status, index, 1),)
     _launch_on(
-        index, "cache_append", "tk_cache_append", k.data_ptr(), _strides_array(ks, kst, 3), v.data_ptr(),
+        index, "cache_append", fn, k.data_ptr(), _strides_array(ks, kst, 3), v.data_ptr(),
         _strides_array(ks, vst, 3), k_pages.data_ptr(), _strides_array(ps, kpst, 3), v_pages.data_ptr(),
         _strides_array(ps, vpst, 3), b, n, hkv, hd, pages, page_size, ptr, stride, width,
         _check_int32(what, "lengths", lengths, index, b), None if new is None else _check_int32(what, "new", new, index, b),
+        *of,
     )
 
 
@@ -687,7 +694,8 @@ def cache_reserve(table, lengths, refs, new, page_size: int):
     free pages are taken, row by row.  Returns an int32 tensor of one entry on the device:
     0 when done; otherwise nothing has changed, and it holds the number of pages that were
     missing, or -1 for a row that would outgrow the table (or a negative length or count).
-    Decided on the device: a captured graph reserves anew at every replay.
+    Decided on the device: a captured graph reserves anew at every replay.  ``cache_append``
+    takes the result and leaves the cache alone where the reservation was refused.
     """
     what = "cache_reserve"
     state = _state_args(what, table, lengths, refs, page_size)
