@@ -38,6 +38,22 @@ def tolerance(out, a, s, dtype, keys, head_dim, vmax, p_step):
     return tol * (1 + u)
 
 
+# fp16 weights go into the products up to 2^15: a weight's step is absolute below 2^-14, half of it 2^-25.
+# paged_attention: relative to the largest weight 2^-25 / 2^15.  window_attention's reference lies 7 below the
+# largest score of the tile that set it, which no later weight undercuts: 2^-25 / 2^7 of the largest weight.
+SMALLEST = {"paged": 2.0 ** -40, "window": 2.0 ** -32}
+
+
+def small_weight_tolerance(out, a, s, dtype, keys, head_dim, vmax, p_step, kind):
+    """As `tolerance`, with what a key's weight can lose below fp16's normal range."""
+    u = HALF_STEP[dtype]
+    weight = p_step + head_dim * 2.0 ** -24 * s[:, None] + 2.0 ** -20 + keys * 2.0 ** -24
+    tol = u * out.abs() + 2 * a * weight + 2.0 ** -24
+    if dtype == torch.float16:
+        tol = tol + 2 * keys * SMALLEST[kind] * vmax
+    return tol * (1 + u)
+
+
 def window_seen(sq, sk, window, sinks, valid=None):
     pos = torch.arange(sk - sq, sk)[:, None]
     j = torch.arange(sk)[None, :]

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from conftest import seeded
-from serving_reference import Book, paged_reference, window_reference
+from serving_reference import HALF_STEP, Book, attend, paged_reference, small_weight_tolerance, window_reference, window_seen
 from tkmi import ops
 
 pytestmark = pytest.mark.gpu
@@ -348,6 +348,87 @@ def test_paged_many_sequences_of_which_some_are_long(b, hkv, longest):
     q = seeded(b, 2 * hkv, 64, dtype=BF16, seed=18)
     _check_paged(q, k, v, table, lens)
     _check_paged(q, k, v, table, lens, window=8200, sinks=3)
+
+
+# ------------------------------------- weights below fp16's normal range, scores past its integers --
+
+
+def _sinks_and_small(n, hd, low, seed, every=None):
+    """One query; key 0 (and each `every`-th) of score 0 and values 0, the others of score ln(low) and values
+    from 1 to 2 (1024 to 2048)."""
+    q, k = torch.zeros(hd, dtype=F16), torch.zeros(n, hd, dtype=F16)
+    q[0] = 1.0
+    k[:, 0] = math.log(low)
+    v = 1 + seeded(n, hd, dtype=F16, seed=seed).abs().clamp_max(1)
+    k[::every or n, 0] = 0
+    v[::every or n] = 0
+    return q, k, v * 1024 if every else v
+
+
+# none is a power of two: a weight lands between two steps of fp16
+SMALL = [2.0 ** -13.7, 2.0 ** -24.5, 2.0 ** -25.2, 2.0 ** -27.6]
+
+
+@pytest.mark.parametrize("low", SMALL)
+@pytest.mark.parametrize("form", ["whole", "split", "invariant"])
+def test_paged_small_weights(low, form):
+    """Weights that only together matter: 3000 tokens in each of 130 sequences, one of them of weight 1; 100000 in one
+    sequence with a weight of 1 in every tile, so in every share of its keys."""
+    hd, ps, dtype = 64, 64, F16
+    n, batch, every = (3000, 130, None) if form == "whole" else (100000, 1, 32)
+    q, k, v = _sinks_and_small(n, hd, low, 90, every)
+    pages = -(-n // ps)
+    kp, vp = (torch.cat([t, t.new_full((-n % ps, hd), float("nan"))]).view(pages, 1, ps, hd) for t in (k, v))
+    table = torch.arange(pages, dtype=torch.int32).expand(batch, -1).contiguous()
+    got = ops.paged_attention(q.expand(batch, 1, -1).contiguous().to(DEV), kp.to(DEV), vp.to(DEV), table.to(DEV),
+                              torch.full((batch,), n, dtype=torch.int32, device=DEV), 1.0, batch_invariant=form == "invariant")
+    o, a, s = attend(q[None], k, v, 1.0, torch.ones(1, n, dtype=torch.bool))
+    tol = small_weight_tolerance(o, a, s, dtype, n, hd, float(v.max()), HALF_STEP[dtype], "paged")
+    _inside(got, o.expand(batch, -1), tol.expand(batch, -1))
+
+
+@pytest.mark.parametrize("low", SMALL)
+@pytest.mark.parametrize("hd", [64, 256])
+def test_window_small_weights(low, hd):
+    """2 rows (keys over workgroups) and 40 (in workgroups of 128 rows, one after the other) of 20000 such keys."""
+    n, dtype = 20000, F16
+    q1, k, v = _sinks_and_small(n, hd, low, 91)
+    for sq, invariant in ((2, False), (2, True), (40, False), (40, True)):
+        q = q1.expand(sq, hd).contiguous()
+        got = ops.window_attention(q[None, None].to(DEV), k[None, None].to(DEV), v[None, None].to(DEV), 1.0, n,
+                                   batch_invariant=invariant)[0]
+        o, a, s = attend(q, k, v, 1.0, window_seen(sq, n, n, 0))
+        tol = small_weight_tolerance(o, a, s, dtype, n, hd, 2.0, HALF_STEP[dtype], "window")
+        _inside(got, o, tol)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("factor", [2.0 ** 8, 2.0 ** 11, 2.0 ** 12])
+def test_scores_of_many_millions(sign, factor):
+    """Scores of 2^21 to 2^26, of either sign, the best one ahead by 64 * factor: its key's values are the row."""
+    n, hd, ps = 900, 64, 32
+    c = torch.randint(129, 255, (n,), generator=torch.Generator().manual_seed(92))
+    c[611] = 255 if sign > 0 else 128
+    for dtype in (F16, BF16):
+        q = torch.full((hd,), 2.0 ** 10, dtype=dtype)
+        k = (sign * c * (factor / 2 ** 10))[:, None].expand(n, hd).to(dtype).contiguous()  # 8 bits: exact
+        v = seeded(n, hd, dtype=dtype, seed=93)
+        want = v[611].double()[None]
+        # the weight rounded and its sum not, and the output rounded
+        tol = 2.01 * HALF_STEP[dtype] * want.abs() + 2.0 ** -24
+        kp, vp = (torch.cat([t, t.new_zeros(-n % ps, hd)]).view(-1, 1, ps, hd).to(DEV) for t in (k, v))
+        table = torch.arange(kp.shape[0], dtype=torch.int32, device=DEV)
+        for invariant in (False, True):
+            for batch in (1, 130):
+                got = ops.paged_attention(q.expand(batch, 1, hd).contiguous().to(DEV), kp, vp,
+                                          table.expand(batch, -1).contiguous(),
+                                          torch.full((batch,), n, dtype=torch.int32, device=DEV), 1.0,
+                                          batch_invariant=invariant)
+                _inside(got, want.expand(batch, -1), tol.expand(batch, -1))
+            for sq in (1, 40):
+                got = ops.window_attention(q.expand(1, 1, sq, hd).contiguous().to(DEV), k[None, None].to(DEV),
+                                           v[None, None].to(DEV), 1.0, n, batch_invariant=invariant)[0]
+                _inside(got[-1:], want, tol)
 
 
 # ------------------------------------------------------------------- cache --

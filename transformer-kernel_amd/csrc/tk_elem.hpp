@@ -54,4 +54,21 @@ struct Elem<bf16> {
   }
 };
 
+// Softmax weights are 2^(x - m), x a score in units of log2 and m a row's reference, the same for O and the sums, so
+// that it cancels.  fp16 holds no more than 2^16 and rounds with fewer bits below 2^-14, in steps of 2^-24: with m the
+// largest score itself 100000 weights of 2^-25 beside one of 1 would all be 0.  So m lies UP below the largest score:
+// weights up to 2^UP.  bf16 has fp32's exponents and needs none of it.  `top` is raw: log2 scores are raw * c, c = s[0].
+// For fp16 m is rounded up (s[1] and s[2]: the next numbers above and below c), so that no weight passes 2^UP where
+// the scores are so large that half a step of m is one and more.
+template <typename T, int UP>
+__device__ __forceinline__ float weight_ref(float top, const float (&s)[3]) {
+  if constexpr (__is_same(T, f16)) return fmaxf(fmaf(top, s[1], -(float)UP), fmaf(top, s[2], -(float)UP));
+  else return top * s[0];
+}
+inline void set_scales(float (&s)[3], float scale) {
+  s[0] = scale * 1.4426950408889634f;
+  s[1] = __builtin_nextafterf(s[0], INFINITY);
+  s[2] = __builtin_nextafterf(s[0], 0.f);
+}
+
 }  // namespace tk

@@ -1,9 +1,10 @@
 // Attention whose keys are split over workgroups: what they leave behind, and the launch that joins it.
 //
 // A row is one query of one head.  Split s of row r leaves, in a slot of its own, its unnormalised
-// output O (fp32, hd values) relative to its running maximum m (in units of log2), and
-// {m, sum of weights}; a split that saw no key leaves m = -inf and no O.  The row is sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s
-// with m the largest m_s, and zeros where nothing was seen.
+// output O (fp32, hd values) relative to its reference m (weight_ref: in units of log2, a little
+// below its largest score), and {m, sum of weights}; a split that saw no key leaves m = -inf and no
+// O.  The row is sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s with m the largest m_s, and zeros where
+// nothing was seen.
 #pragma once
 #include "tk_elem.hpp"
 
@@ -25,7 +26,7 @@ struct JoinArgs {
 
 constexpr int kJoinWaves = 4;
 
-// A result in the making: maximum, sum of weights and 4 columns of O relative to the maximum.
+// A result in the making: reference, sum of weights and 4 columns of O relative to the reference.
 struct JoinPart {
   float m, l;
   f32x4 o;

@@ -23,9 +23,10 @@
 // Where the sequences and key heads alone would leave CUs idle, every sequence's keys are split
 // over workgroups (paged_share), and a second launch joins their results (tk_join.hpp).
 //
-// Numerics: fp32 scores, maxima, sums and O.  P is rounded to 16 bits for the product: fp16
-// (half a step 2^-11 of the weight) as it is; bf16 (2^-8) as the sum of two bf16 numbers, whose
-// second product the idle matrix cores do for nothing.
+// Numerics: fp32 scores, references, sums and O.  P is rounded to 16 bits for the product: bf16 (half a step
+// 2^-8 of the weight) as the sum of two bf16 numbers, whose second product the idle matrix cores do for
+// nothing; fp16 as it is, 2^15 at most (weight_ref): half a step is 2^-11 of weights down to 2^-29 of the
+// wave's largest, and 2^-40 of that one below.
 #include "tk_join.hpp"
 
 namespace tk {
@@ -52,7 +53,7 @@ struct PagedArgs {
   bool fill;    // paged_share: as many shares as there are workers
   int least;    // tiles of the smallest share
   int fixed;    // > 0: shares of this many tiles, workers / batch of them per sequence
-  float scale_log2;
+  float scales[3];  // weight_ref
 };
 
 // The tiles of 32 keys that hold visible ones: those of the sinks, then those of the window.
@@ -254,7 +255,7 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
 #pragma unroll
   for (int m = 0; m < CW; ++m) acc[m] = f32x4{};
   float m_run = -INFINITY, l_run = 0.f;
-  const float cs = p.scale_log2;
+  const float cs = p.scales[0];
 
   // One step: the keys from k0 on are in kf and vf; those from `k0n` on follow, if there are more.
   auto step = [&](auto more, int k0, int p0, int p1, int k0n, int p0n, int p1n) {
@@ -285,7 +286,7 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
     }
     float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    const float m_new = fmaxf(m_run, quad_max(mx) * cs);
+    const float m_new = fmaxf(m_run, weight_ref<T, 15>(quad_max(mx), p.scales));
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
     m_run = m_new;
@@ -349,7 +350,7 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
     step(BoolOf<false>(), k0, p0, p1, 0, -1, -1);
   }
 
-  // ---- the waves' results, rescaled to the common maximum and added in wave order ----
+  // ---- the waves' results, rescaled to the largest reference and added in wave order ----
   l_run = quad_sum(l_run);
   constexpr int VW = CW < 4 ? CW : 4;  // neighbouring columns written at once
   typedef float vec __attribute__((ext_vector_type(VW)));
@@ -621,7 +622,7 @@ extern "C" int tk_paged_attn(const void* q, const int64_t* q_strides, const void
   p.fill = plan.fill;
   p.least = (int)kPagedLeast;
   p.fixed = (int)plan.fixed;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  set_scales(p.scales, scale);
   hipStream_t st = as_stream(stream);
   return dtype == TK_F16 ? launch_paged<f16>(p, per_seq * plan.workers, st)
                          : launch_paged<bf16>(p, per_seq * plan.workers, st);

@@ -11,13 +11,14 @@
 //
 // As in tk_attention.hip a wave computes S^T = K . Q^T (a lane holds one query row's scores, the
 // running maximum is one lane-pair exchange) and O^T = V^T . P^T with the accumulator's keys as
-// the product's k slots and V^T from transposed LDS reads.  The running maximum is raised only
-// when a tile exceeds it by more than 2^8: O and the sums may hold weights up to 256, harmless in
-// fp32 and in 16-bit P, and the rescale of O is skipped on most tiles.
+// the product's k slots and V^T from transposed LDS reads.  The weights' reference (weight_ref) is
+// raised only when a tile's largest score passes that of the tile that set it by more than 2^8, harmless
+// in fp32 and in 16-bit P, and the rescale of O is skipped on most tiles.
 //
-// Numerics: fp32 scores, maxima, sums, O; P rounded to the inputs' type for the product (half a
-// step: fp16 2^-11, bf16 2^-8 of the weight), the sum taken of the rounded weights, so that they
-// add up to 1.
+// Numerics: fp32 scores, references, sums, O; P rounded to the inputs' type for the product, the sum taken
+// of the rounded weights, so that they add up to 1.  Half a step is 2^-8 of the weight in bf16; in fp16,
+// with weights up to 2^15, 2^-11 of those down to 2^-21 of the largest when the reference was set, and 2^-32
+// of that one below.
 #include "tk_attn_tile.hpp"
 #include "tk_join.hpp"
 
@@ -38,7 +39,7 @@ struct WindowArgs {
   int splits, per_split;  //   and key tiles of a workgroup
   float* part;            // its results where splits > 1 (tk_join.hpp)
   float* stats;
-  float scale_log2;
+  float scales[3];        // weight_ref
 };
 
 // The key tiles that rows at positions [first, last] see: those of the sinks, then those of the windows.
@@ -150,7 +151,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  const float cs = p.scale_log2;
+  const float cs = p.scales[0];
 
   copy(0, lds0);
   for (int t = 0; t < tiles.n; ++t) {
@@ -201,7 +202,7 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16 * NB; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
-    const float m_tile = pair_max(mx) * cs;
+    const float m_tile = weight_ref<T, 7>(pair_max(mx), p.scales);
     if (__ballot(m_tile > m_run + 8.f) != 0ull) {
       const float m_new = fmaxf(m_run, m_tile);
       const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
@@ -345,7 +346,7 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  const float cs = p.scale_log2;
+  const float cs = p.scales[0];
 
   for (; t < t_end; t += NW) {
     const int k0 = tiles.key(t);
@@ -381,7 +382,7 @@ __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16 * NB; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
-    const float m_tile = pair_max(mx) * cs;
+    const float m_tile = weight_ref<T, 7>(pair_max(mx), p.scales);
     if (__ballot(m_tile > m_run + 8.f) != 0ull) {
       const float m_new = fmaxf(m_run, m_tile);
       const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
@@ -651,7 +652,7 @@ extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const voi
   p.hd = (int)head_dim;
   p.window = (int)at_most(window, k_len);
   p.sinks = (int)at_most(sinks, k_len);
-  p.scale_log2 = scale * 1.4426950408889634f;
+  set_scales(p.scales, scale);
   const WindowPlan plan =
       window_plan(batch * heads, p.group, q_len, k_len, p.window, p.sinks, head_dim, batch_invariant != 0);
   const int64_t rows = batch * heads * q_len, need = window_workspace(plan, rows, head_dim);
