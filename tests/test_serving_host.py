@@ -147,6 +147,15 @@ def test_launches_of_too_many_workgroups_are_refused():
     assert lib.tk_cache_free(*state, 16, 1 << 24, None) == -1
 
 
+def test_a_join_of_too_many_workgroups_is_refused_before_the_first_launch():
+    """2^22 workgroups attend, but 2^24 would join them: the refusal (and not what a launch says here)."""
+    call = dict(b=65536, h=32, hkv=32, hd=128, pages=8, ps=16, width=128, stride=128, most=2048, invariant=1, ws=16)
+    need = _lib.load().tk_paged_attn_workspace(65536, 32, 32, 128, 2048, 0, 0, 1)
+    assert need > 0 and _paged(**call, size=need - 1) in (-1, -2)
+    assert _paged(**call, size=need) == -2
+    assert "too many workgroups" in _lib.load().tk_last_error_string().decode()
+
+
 def test_wrappers_refuse_on_the_cpu():
     half = torch.zeros(1, 2, 4, 64, dtype=torch.float16)
     table, vec = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)

@@ -90,14 +90,19 @@ __global__ __launch_bounds__(kJoinWaves * 64) void split_join_kernel(JoinArgs p)
   for (int e = 0; e < 4; ++e) out[e] = (T)(r.l == 0.f ? 0.f : r.o[e] / r.l);
 }
 
+// Few splits: a wave per row.  one_order: the tree of the groups, in which splits that a longer table adds
+// (empty ones) change no bit.
+inline bool join_grouped(int64_t splits, bool one_order) { return one_order || splits > 16; }
+
+// Workgroups of the join; above kMaxGroups the whole call is to be refused, before its first launch.
+inline int64_t join_grid(int64_t rows, int64_t hd, int64_t splits, bool one_order) {
+  return join_grouped(splits, one_order) ? rows * ((hd + 15) / 16) : (rows + kJoinWaves - 1) / kJoinWaves;
+}
+
 template <typename T>
 int launch_join(const char* fn, const JoinArgs& p, bool one_order, hipStream_t st) {
-  // Few splits: a wave per row.  one_order: the tree of the groups, in which splits that a longer table adds
-  // (empty ones) change no bit.
-  const bool grouped = one_order || p.splits > 16;
-  const int64_t grid = grouped ? p.rows * ((p.hd + 15) / 16) : (p.rows + kJoinWaves - 1) / kJoinWaves;
-  TK_REQUIRE(grid <= kMaxGroups, TK_ERR_UNSUPPORTED, "%s: too many rows", fn);
-  const dim3 g((unsigned)grid), blk(kJoinWaves * 64);
+  const bool grouped = join_grouped(p.splits, one_order);
+  const dim3 g((unsigned)join_grid(p.rows, p.hd, p.splits, one_order)), blk(kJoinWaves * 64);
   if (grouped) hipLaunchKernelGGL((split_join_kernel<T, true>), g, blk, 0, st, p);
   else hipLaunchKernelGGL((split_join_kernel<T, false>), g, blk, 0, st, p);
   return check_launch(fn);

@@ -581,8 +581,10 @@ extern "C" int tk_paged_attn(const void* q, const int64_t* q_strides, const void
   if (batch_invariant && max_length < table_width * page_size) max_length = table_width * page_size;
   const int64_t per_seq = per_sequence(heads, kv_heads);
   const PagedPlan plan = paged_plan(batch, per_seq, max_length, window, sinks, batch_invariant != 0);
-  TK_REQUIRE(per_seq * plan.workers <= kMaxGroups, TK_ERR_UNSUPPORTED, "tk_paged_attn: too many workgroups");
   const int64_t need = paged_workspace(plan, batch, heads, head_dim);
+  TK_REQUIRE(per_seq * plan.workers <= kMaxGroups &&
+                 (need == 0 || join_grid(batch * heads, head_dim, plan.workers / batch, plan.fixed > 0) <= kMaxGroups),
+             TK_ERR_UNSUPPORTED, "tk_paged_attn: too many workgroups");
   TK_REQUIRE(need == 0 || (workspace && al(workspace, 16) && workspace_bytes >= need), TK_ERR_ARG,
              "tk_paged_attn: workspace of %lld bytes, 16-byte aligned, needed", (long long)need);
   PagedArgs p{};

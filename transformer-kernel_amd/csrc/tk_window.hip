@@ -519,9 +519,9 @@ WindowPlan window_plan(int64_t bh, int64_t group, int64_t q_len, int64_t k_len, 
   // the sinks and the windows may begin and end inside tiles
   const int64_t tiles = (keys + kSplitKeys - 1) / kSplitKeys + 2;
   if (batch_invariant) return {true, unit, blocks, 1, tiles};
-  // A block's keys go to several workgroups only up to one workgroup per CU, in shares of three tiles a wave or
-  // more: past that the launch that joins them costs more (10 x 2 heads of 128, 735 rows: whole 20 us, in two
-  // 38; 3 heads of 64, 923 rows, window 2920: 18 us in eight shares, 34 whole).
+  // A block's keys go to several workgroups only up to one workgroup per CU (8192 rows to be joined at most),
+  // in shares of three tiles a wave or more: past that the launch that joins them costs more (10 x 2 heads of
+  // 128, 735 rows: whole 20 us, in two 38; 3 heads of 64, 923 rows, window 2920: 18 us in eight shares, 34 whole).
   const int64_t want = blocks < 256 ? 256 / blocks : 1;
   int64_t per = (tiles + want - 1) / want;
   per = (per + kWindowWaves - 1) / kWindowWaves * kWindowWaves;
