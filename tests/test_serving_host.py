@@ -2,9 +2,13 @@
 
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from conftest import PKG_PARENT
 from tkmi import _lib, ops
 
 S3 = _lib.strides([64, 64, 64])
@@ -154,6 +158,20 @@ def test_a_join_of_too_many_workgroups_is_refused_before_the_first_launch():
     assert need > 0 and _paged(**call, size=need - 1) in (-1, -2)
     assert _paged(**call, size=need) == -2
     assert "too many workgroups" in _lib.load().tk_last_error_string().decode()
+
+
+def test_import_needs_no_gpu_build_of_torch():
+    """A torch without a GPU backend has no current raw stream: the package imports, its operators say what they need."""
+    code = ("import torch, sys\n"
+            "del torch._C._cuda_getCurrentRawStream\n"
+            "sys.path.insert(0, %r)\n"
+            "import tkmi\n"
+            "v = torch.zeros(1, dtype=torch.int32)\n"
+            "try: tkmi.ops.cache_free(v[None], v, v, v, 16)\n"
+            "except RuntimeError as e: assert 'GPU only' in str(e)\n"
+            "else: raise SystemExit(2)\n") % str(PKG_PARENT)
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-500:]
 
 
 def test_wrappers_refuse_on_the_cpu():
