@@ -442,7 +442,8 @@ int tk_forward(const tk_model *model, const void *x, void *out, int64_t batch, i
  * new token over it.  All of them take 16-bit tensors of one dtype (TK_F16 or TK_BF16),
  * head_dim a multiple of 8 up to 256, and rows of 16-byte vectors (base 16-byte aligned,
  * strides multiples of 8 elements; out: 8-byte in tk_window_attn, any in tk_paged_attn).
- * heads is a multiple of kv_heads; head h reads key head h / (heads / kv_heads).
+ * heads is a multiple of kv_heads; head h reads key head h / (heads / kv_heads).  scale is
+ * positive and at most 2.3e38.
  * No counterpart in the reference, which recomputes whole sequences with full causal
  * attention (src/kernels.py:250-294).
  */
@@ -453,7 +454,7 @@ int tk_forward(const tk_model *model, const void *x, void *out, int64_t batch, i
  * j < sinks, and key_valid[b * key_valid_stride + j] (nullable) is set.  window >= 1; one of
  * k_len or more is plain causal attention.  A query that sees nothing gets 0.
  * q [batch, heads, q_len, head_dim], k and v [batch, kv_heads, k_len, head_dim], out as q:
- * element strides {b, h, s} in *_strides[3].  scale > 0.  What K and V hold at keys that
+ * element strides {b, h, s} in *_strides[3].  What K and V hold at keys that
  * are not valid has no effect; at valid ones it must be finite.
  * Launches with few query rows split their keys over workgroups; batch_invariant: not so, a
  * sequence's bits do not depend on the rest of the batch.  workspace:

@@ -124,6 +124,12 @@ def test_cache_calls_refuse():
     assert lib.tk_cache_workspace(-1, 4, 0) == -1 and lib.tk_cache_workspace(2, 8, 3) >= 4 * (6 + 16)
 
 
+@pytest.mark.parametrize("scale,code", [(2.3e38, 0), (2.36e38, -1), (3.0e38, -1), (-1.0, -1), (1e-45, 0)])
+def test_scales_whose_log2_units_are_infinite_are_refused(scale, code):
+    """Scores are scaled by scale * log2(e); an infinite factor would make a score of 0 NaN."""
+    assert _window(b=0, scale=scale) == code and _paged(b=0, scale=scale) == code
+
+
 def test_append_with_a_status_refuses():
     """As without one, and a status that is not there."""
     lib = _lib.load()

@@ -65,6 +65,7 @@ __device__ __forceinline__ float weight_ref(float top, const float (&s)[3]) {
   if constexpr (__is_same(T, f16)) return fmaxf(fmaf(top, s[1], -(float)UP), fmaf(top, s[2], -(float)UP));
   else return top * s[0];
 }
+constexpr float kMaxScale = 2.3e38f;  // c stays finite: an infinite one would make a score of 0 NaN
 inline void set_scales(float (&s)[3], float scale) {
   s[0] = scale * 1.4426950408889634f;
   s[1] = __builtin_nextafterf(s[0], INFINITY);

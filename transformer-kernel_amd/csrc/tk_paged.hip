@@ -563,7 +563,8 @@ extern "C" int tk_paged_attn(const void* q, const int64_t* q_strides, const void
   TK_REQUIRE(batch == 0 || table_width * page_size <= (1ll << 34) / batch, TK_ERR_UNSUPPORTED,
              "tk_paged_attn: a table of more than 2^34 tokens");
   TK_REQUIRE(batch <= 1 || table_stride >= table_width, TK_ERR_ARG, "tk_paged_attn: table_stride < table_width");
-  TK_REQUIRE(scale > 0.f && scale <= 3.0e38f, TK_ERR_ARG, "tk_paged_attn: scale must be positive and finite");
+  TK_REQUIRE(scale > 0.f && scale <= kMaxScale, TK_ERR_ARG,
+             "tk_paged_attn: scale must be positive and at most 2.3e38");
   if (batch == 0 || heads == 0 || head_dim == 0) return TK_OK;
   TK_REQUIRE(q && out && lengths && q_strides && k_strides && v_strides && o_strides &&
                  ((k_pages && v_pages) || pages == 0) && (table || table_width == 0),

@@ -622,7 +622,7 @@ extern "C" int tk_window_attn(const void* q, const int64_t* q_strides, const voi
   TK_REQUIRE(dtype == TK_F16 || dtype == TK_BF16, TK_ERR_ARG, "%s: dtype %d is not TK_F16 or TK_BF16", fn, dtype);
   const int rc = check_window_shape(fn, batch, heads, kv_heads, q_len, k_len, head_dim, window, sinks);
   if (rc != TK_OK) return rc;
-  TK_REQUIRE(scale > 0.f && scale <= 3.0e38f, TK_ERR_ARG, "%s: scale must be positive and finite", fn);
+  TK_REQUIRE(scale > 0.f && scale <= kMaxScale, TK_ERR_ARG, "%s: scale must be positive and at most 2.3e38", fn);
   if (batch == 0 || heads == 0 || q_len == 0 || head_dim == 0) return TK_OK;
   TK_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides && o_strides, TK_ERR_ARG, "%s: null pointer", fn);
   TK_REQUIRE(key_valid == nullptr || key_valid_stride >= k_len, TK_ERR_ARG, "%s: key_valid_stride=%lld < k_len", fn,
