@@ -204,6 +204,21 @@ def test_window_short_queries_leave_what_lies_around_them():
     assert bool((buf == 7.0).all())
 
 
+@pytest.mark.parametrize("b,h,hkv,sq", [(1, 4, 1, 8), (1, 66, 1, 1), (1, 40, 1, 3), (3, 66, 1, 1)])
+@pytest.mark.parametrize("hd", [24, 64, 104, 256])
+def test_window_short_queries_of_one_group_partly_masked(b, h, hkv, sq, hd):
+    """Groups that span several blocks of 32 rows: rows that see some of the keys, and (last sequence of several) none."""
+    sk = sq + 170
+    q, k, v = _window_inputs(b, h, hkv, sq, sk, hd, F16 if sq % 2 else BF16, seed=sq + h)
+    valid = torch.rand(b, sk, generator=torch.Generator().manual_seed(h)) > 0.3
+    valid[0, sk - sq - 40:sk - 2] = False  # all that the window holds but for the last keys
+    if b > 1:
+        valid[-1] = False
+    bad = ~valid[:, None, :, None].expand_as(k)
+    out = _check_window(q, k.masked_fill(bad, float("nan")), v.masked_fill(bad, float("inf")), 75, 3, valid)
+    assert bool(out[:, 0].any()) and (b == 1 or not out[:, -1].any())
+
+
 # ------------------------------------------------------------------- paged --
 
 
