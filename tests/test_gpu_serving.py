@@ -219,6 +219,31 @@ def test_window_short_queries_of_one_group_partly_masked(b, h, hkv, sq, hd):
     assert bool(out[:, 0].any()) and (b == 1 or not out[:, -1].any())
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_window_offsets_past_32_bits(hd):
+    """Rows and sequences of q, k, v and out that lie past 2^32 elements."""
+    n, far = 2100, 2 ** 21
+    buf = torch.empty(n * far, dtype=BF16, device=DEV)
+
+    def rows(count, at):
+        return buf.as_strided((1, 2, count, hd), (0, 2 ** 9, far, 1), at)
+
+    for sq, invariant in ((1, False), (40, False), (300, True)):
+        q, k, v = _window_inputs(1, 2, 2, sq, n, hd, BF16, seed=hd + sq)
+        qd, kd, vd = (rows(t.shape[2], at).copy_(t) for t, at in ((q, 0), (k, 2 ** 18), (v, 2 ** 19)))
+        out = buf.as_strided((1, sq, 2 * hd), (0, far, 1), (n - sq) * far + 2 ** 20)
+        ops.window_attention(qd, kd, vd, 0.1, 1500, sinks=5, out=out, batch_invariant=invariant)
+        want, tol = window_reference(q, k, v, 0.1, 1500, 5)
+        _inside(out, want, tol)
+    # two sequences that lie so far apart
+    q, k, v = _window_inputs(2, 2, 2, 50, 200, hd, BF16, seed=hd)
+    qd, kd, vd = (buf.as_strided(t.shape, (2 ** 32 + 8, t.shape[2] * hd, hd, 1), at).copy_(t)
+                  for t, at in ((q, 0), (k, 2 ** 18), (v, 2 ** 19)))
+    for invariant in (False, True):
+        want, tol = window_reference(q, k, v, 0.1, 70, 3)
+        _inside(ops.window_attention(qd, kd, vd, 0.1, 70, sinks=3, batch_invariant=invariant), want, tol)
+
+
 # ------------------------------------------------------------------- paged --
 
 
