@@ -427,6 +427,22 @@ def test_paged_small_weights(low, form):
     _inside(got, o.expand(batch, -1), tol.expand(batch, -1))
 
 
+@pytest.mark.parametrize("dtype,p_step", [(F16, 2.0 ** -22), (BF16, 2.0 ** -16)])
+def test_paged_weights_are_two_numbers(dtype, p_step):
+    """The weights' rounding does not show: few keys and narrow heads, so that the bound is the output's rounding."""
+    lengths = [2, 7, 20, 40, 64, 90]
+    for hd in (8, 16):
+        k, v, table, lens = _cache(lengths, 1, hd, 16, dtype, seed=94)
+        q = seeded(len(lengths), 16, hd, dtype=dtype, seed=95)
+        got = ops.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), lens.to(DEV), 0.3)
+        for b, n in enumerate(lengths):
+            ids = table[b, :-(-n // 16)].long()
+            kk, vv = (t[ids, 0].reshape(-1, hd)[:n] for t in (k, v))
+            o, a, s = attend(q[b], kk, vv, 0.3, torch.ones(16, n, dtype=torch.bool))
+            tol = small_weight_tolerance(o, a, s, dtype, n, hd, float(vv.abs().max()), p_step, "paged")
+            _inside(got[b].view(16, hd), o, tol)
+
+
 @pytest.mark.parametrize("low", SMALL)
 @pytest.mark.parametrize("hd", [64, 256])
 def test_window_small_weights(low, hd):

@@ -23,10 +23,10 @@
 // Where the sequences and key heads alone would leave CUs idle, every sequence's keys are split
 // over workgroups (paged_share), and a second launch joins their results (tk_join.hpp).
 //
-// Numerics: fp32 scores, references, sums and O.  P is rounded to 16 bits for the product: bf16 (half a step
-// 2^-8 of the weight) as the sum of two bf16 numbers, whose second product the idle matrix cores do for
-// nothing; fp16 as it is, 2^15 at most (weight_ref): half a step is 2^-11 of weights down to 2^-29 of the
-// wave's largest, and 2^-40 of that one below.
+// Numerics: fp32 scores, references, sums and O.  P goes into the product as the sum of two 16-bit numbers, the
+// second the first one's rounding error; the idle matrix cores do its product for nothing.  What is left is
+// 2^-16 of a weight in bf16; in fp16, where the largest is 2^15 (weight_ref), 2^-22 of weights down to 2^-18 of
+// the wave's largest, and at most 2^-40 of that one below.
 #include "tk_join.hpp"
 
 namespace tk {
@@ -177,7 +177,6 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
   constexpr int KS = DT / 32;   // 32-wide steps of S^T
   constexpr int CW = DT / 16;   // columns of V per lane
   constexpr int DW = CW / 2;    // the same in words
-  constexpr bool SPLIT_P = !__is_same(T, f16);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -301,7 +300,7 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       pf[i] = (T)e[i];
-      if (SPLIT_P) pl[i] = (T)(e[i] - (float)pf[i]);
+      pl[i] = (T)(e[i] - (float)pf[i]);
     }
 #pragma unroll
     for (int m = 0; m < CW; ++m)
@@ -321,7 +320,7 @@ __device__ __forceinline__ void paged_segment(const PagedArgs& p, PagedLds<DT, N
         a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][m >> 1], vf[2 * i][m >> 1], m & 1 ? 0x07060302u : 0x05040100u);
       const x8 va = __builtin_bit_cast(x8, a);
       acc[m] = Elem<T>::mfma16(va, pf, acc[m]);
-      if (SPLIT_P) acc[m] = Elem<T>::mfma16(va, pl, acc[m]);
+      acc[m] = Elem<T>::mfma16(va, pl, acc[m]);
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (decltype(more)::value) load_v(k0n, p0n, p1n);
