@@ -494,7 +494,8 @@ int tk_window_attn(const void *q, const int64_t *q_strides, const void *k,
  * workgroups, longer sequences are attended whole.  batch_invariant: a sequence's bits do
  * not depend on the rest of the batch, table_width or max_length, which then counts (in the
  * workspace's size too) as at least table_width * page_size.  workspace: tk_paged_attn_workspace bytes, 16-byte
- * aligned, this call's own until its launches have run (0 bytes: may be NULL).
+ * aligned, this call's own until its launches have run (0 bytes: may be NULL).  Fewer than 2^24
+ * rows (batch * heads) and at most 2^34 tokens (batch * table_width * page_size) in all.
  */
 int64_t tk_paged_attn_workspace(int64_t batch, int64_t heads, int64_t kv_heads,
                                 int64_t head_dim, int64_t max_length,

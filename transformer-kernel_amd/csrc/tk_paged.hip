@@ -24,8 +24,8 @@
 // over workgroups (paged_share), and a second launch joins their results (tk_join.hpp).
 //
 // Numerics: fp32 scores, references, sums and O.  P goes into the product as the sum of two 16-bit numbers, the
-// second the first one's rounding error; the idle matrix cores do its product for nothing.  What is left is
-// 2^-16 of a weight in bf16; in fp16, where the largest is 2^15 (weight_ref), 2^-22 of weights down to 2^-18 of
+// second the first one's rounding error, whose product the idle matrix cores do (fp16: +1.2 % of the time over 20
+// shapes, 4.18 -> 4.28 us for a single short sequence, nothing where HBM bounds).  What is left is 2^-16 of a weight in bf16; in fp16, where the largest is 2^15 (weight_ref), 2^-22 of weights down to 2^-18 of
 // the wave's largest, and at most 2^-40 of that one below.
 #include "tk_join.hpp"
 

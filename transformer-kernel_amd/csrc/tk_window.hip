@@ -253,9 +253,10 @@ __device__ __forceinline__ void window_body(const WindowArgs& p) {
 // chain each.  32 rows of one head per workgroup, or of a group's heads one after the other; wave w takes
 // every NW-th of its tiles of kSplitKeys keys, into K and V slots of its own, so the loop has no barrier: the
 // next K is copied when the current one's products are done, the next V after P.V.  At the end the waves'
-// (max, sum, O) are merged in wave order.  Tiles of 32 keys leave room for two to six workgroups per CU: 16
-// heads of 64, 619 rows, window 126 9.0 us, with tiles of 64 11.7.  (Two waves of rows per tile, tiles ahead
-// in a second slot: 14.0, and 31 us instead of 38 where a window of 2048 keys makes the chains long.)
+// (reference, sum, O) are merged in wave order.  Tiles of 32 keys leave room for seven workgroups per CU at
+// head_dim 32, four at 64, two at 128 (at 256 one takes 129 KB): 16 heads of 64, 619 rows, window 126 9.0 us, with
+// tiles of 64 11.7.  (Two waves of rows per tile, tiles ahead in a second slot: 14.0, and 31 us instead of 38
+// where a window of 2048 keys makes the chains long.)
 constexpr int kSplitKeys = 32;
 template <typename T, int DT, int NW, bool KMASK>
 __device__ __forceinline__ void window_split_body(const WindowArgs& p) {
