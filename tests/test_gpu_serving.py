@@ -869,6 +869,45 @@ def test_streams_and_two_graphs():
             assert torch.equal(o, want)
 
 
+def test_window_streams_and_graphs():
+    """Keys over workgroups: calls on two streams at once and two graphs replayed in turn, each with a workspace of its
+    own, whatever memory held before; the same bits every time."""
+    k, v = (seeded(1, 2, 9000, 64, dtype=F16, seed=i).to(DEV) for i in (63, 64))
+    qs = [seeded(1, 4, n, 64, dtype=F16, seed=65 + n).to(DEV) for n in (3, 7)]
+
+    def call(q):
+        return ops.window_attention(q, k, v, 0.125, 8000, sinks=5)
+
+    wants = [call(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(5):
+        junk = [torch.full((1 << 20,), float("nan"), device=DEV) for _ in range(4)]
+        del junk  # what the workspaces are made of
+        got = []
+        for s, q in zip(streams, qs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(call(q))
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for g, want in zip(got, wants):
+            assert torch.equal(g, want)
+    graphs = []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = call(q)
+        graphs.append((g, o))
+    for _ in range(3):
+        for _, o in graphs:
+            o.zero_()
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (_, o), q, want in zip(graphs, qs, wants):
+            assert torch.equal(o, want) and torch.equal(call(q), want)
+
+
 def test_wrappers_refuse():
     q = torch.zeros(1, 2, 4, 64, dtype=F16, device=DEV)
     table, vec = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
